@@ -277,6 +277,137 @@ int attn_qkv_gemm_rope_store_kv(const attn_f16_t* x, attn_f16_t* y, const attn_f
                                 size_t num_kv_heads, size_t head_dim, size_t start_pos,
                                 int apply_rotation, hipStream_t stream);
 
+/* ---- Paged KV cache: the decode step of a batch of sequences.  No counterpart
+ * in the reference, which serves one sequence from contiguous cache rows.
+ *
+ * A pool holds num_pages pages per plane (K or V of a layer); a page is page_size
+ * cache rows of num_kv_heads * head_dim fp16 values, rows as in the contiguous
+ * cache: a KVCache whose max_seq_len is num_pages * page_size is such a pool, layer
+ * l's K and V its planes 2 l and 2 l + 1.  Row b of a page table, max_pages int32
+ * entries, names the pages of sequence b in order: its cache row t is row t %
+ * page_size of page table[b][t / page_size].  Entries past a sequence's length are
+ * never read.  All of this is device memory, so lengths and tables may change
+ * between replays of a captured call.  Sizes: num_pages * page_size and max_pages *
+ * page_size at most 2^31 - 1; any page_size.  num_seqs, num_tokens or n == 0 is a
+ * no-op.  Page numbers, sequence numbers, positions and lengths that are out of
+ * range are caught on the device, as said at each call. */
+
+/* RoPE + append of num_tokens new tokens into pages: attn_rope_store_kv for token
+ * t at position positions[t] of sequence seq_ids[t] (NULL: sequence t, one token
+ * each), cache rows in pages.  q rows are q_stride apart, k and v rows k_stride
+ * apart (0 = packed).  q_out != NULL: the (rotated) queries go there, packed
+ * [num_tokens][num_heads][head_dim], and q is only read; NULL: in place, as
+ * attn_rope_store_kv.  apply_rotation == 0: K and V (and q, to q_out) copied.
+ * Values equal attn_rope_store_kv's bit for bit.  cos/sin are
+ * [max_seq_len][head_dim/2].  A token with a negative position (a padded batch),
+ * one at or past max_seq_len or its table row's pages, or with a sequence or page
+ * number out of range is left out: nothing of it is written.  No two tokens may
+ * name one cache row. */
+int attn_paged_rope_store_kv(attn_f16_t* q, const attn_f16_t* k, const attn_f16_t* v,
+                             attn_f16_t* q_out, attn_f16_t* k_pages, attn_f16_t* v_pages,
+                             const attn_f16_t* cos_table, const attn_f16_t* sin_table,
+                             const int32_t* page_table, const int32_t* seq_ids,
+                             const int32_t* positions, size_t num_tokens, size_t num_seqs,
+                             size_t max_pages, size_t num_pages, size_t page_size,
+                             size_t max_seq_len, size_t num_heads, size_t num_kv_heads,
+                             size_t head_dim, size_t q_stride, size_t k_stride,
+                             int apply_rotation, hipStream_t stream);
+
+/* Decode attention of one new token per sequence over its first kv_lens[b] cached
+ * rows (the paged, batched form of attn_decode; lengths are cut at max_pages *
+ * page_size).  q rows are q_stride apart (0 = packed); out is packed
+ * [num_seqs][num_heads][head_dim].  A sequence of length 0 or less keeps its
+ * output row; one whose table names a page out of range gets NaN.  head_dim up to
+ * 256; num_heads a multiple of num_kv_heads.  workspace:
+ * attn_paged_decode_workspace_bytes bytes, 16-byte aligned, any contents; calls
+ * that share one must be ordered (one stream, or graphs replayed in order). */
+size_t attn_paged_decode_workspace_bytes(size_t num_seqs, size_t num_heads, size_t num_kv_heads,
+                                         size_t head_dim);
+int attn_paged_decode(const attn_f16_t* q, const attn_f16_t* k_pages, const attn_f16_t* v_pages,
+                      attn_f16_t* out, const int32_t* page_table, const int32_t* kv_lens,
+                      size_t num_seqs, size_t max_pages, size_t num_pages, size_t page_size,
+                      size_t num_heads, size_t num_kv_heads, size_t head_dim, size_t q_stride,
+                      void* workspace, hipStream_t stream);
+
+/* Page management.  ref_counts[p] is the number of table rows that name page p (0:
+ * free); seq_lens[b] the tokens of sequence b, whose row names ceil(seq_lens[b] /
+ * page_size) pages.  A pool is num_planes planes, plane_stride elements apart (0 =
+ * num_pages * page_elems), of num_pages pages of page_elems elements; the calls
+ * below move pages in every plane at once.  Calls on one state must be ordered.
+ *
+ * attn_pages_copy: pages src[i] -> dst[i], i < n.  Pairs with a number out of range
+ * are left out.  No page may be in dst twice, nor in both lists. */
+int attn_pages_copy(attn_f16_t* pool, size_t num_planes, size_t plane_stride, size_t page_elems,
+                    const int32_t* src, const int32_t* dst, size_t n, size_t num_pages,
+                    hipStream_t stream);
+
+/* Cuts sequence b to keep_lens[b] tokens (NULL: 0 for every sequence; a negative
+ * entry or one not below the length leaves the sequence alone): the pages past them
+ * lose a reference.  Table entries stay as they were. */
+int attn_pages_free(int32_t* page_table, int32_t* seq_lens, const int32_t* keep_lens,
+                    int32_t* ref_counts, size_t num_seqs, size_t max_pages, size_t num_pages,
+                    size_t page_size, hipStream_t stream);
+
+/* Row i of the destination table becomes a fork of source row parents[i]: it names
+ * the same pages, which gain a reference, and has the same length; nothing is copied
+ * until one of them grows.  Left alone: rows whose parent is negative or not below
+ * num_src, and rows that hold a sequence (dst_lens[i] > 0).  The two tables (both
+ * max_pages wide) may be one, dst_lens then src_lens and num_dst num_src; rows whose
+ * parent has a parent in the same call are then left alone. */
+int attn_pages_fork(const int32_t* src_table, const int32_t* src_lens, int32_t* dst_table,
+                    int32_t* dst_lens, const int32_t* parents, int32_t* ref_counts, size_t num_src,
+                    size_t num_dst, size_t max_pages, size_t num_pages, size_t page_size,
+                    hipStream_t stream);
+
+/* Sequence b grows by grow[b] tokens (0 or less: not at all).  New pages are the
+ * lowest free ones, in the order of the rows.  A row whose last page is partly filled
+ * and named by other rows too gets a copy of it (its first new page), so the new
+ * tokens' cache rows belong to it alone.  status[0]: the pages the pool lacks, status[1]:
+ * the rows that would pass max_pages (status[0] is then 0); unless both are 0 nothing
+ * else has changed.  workspace: attn_pages_workspace_bytes(num_seqs, num_pages) bytes,
+ * 4-byte aligned, any contents. */
+size_t attn_pages_workspace_bytes(size_t num_seqs, size_t num_pages);
+int attn_pages_grow(attn_f16_t* pool, size_t num_planes, size_t plane_stride, size_t page_elems,
+                    int32_t* page_table, int32_t* seq_lens, const int32_t* grow,
+                    int32_t* ref_counts, int32_t* status, size_t num_seqs, size_t max_pages,
+                    size_t num_pages, size_t page_size, void* workspace, hipStream_t stream);
+
+/* Moves the used pages to the front of the pool: with *num_used pages in use, those at
+ * num_used and above go, in order, to the free pages below, in order.
+ * page_table_out and ref_counts_out receive the new state (table entries within the
+ * sequences' lengths); each may be its input or not overlap it.  num_seqs must cover every
+ * row that names a page.  workspace as attn_pages_grow's. */
+int attn_pages_compact(attn_f16_t* pool, size_t num_planes, size_t plane_stride, size_t page_elems,
+                       const int32_t* page_table, const int32_t* seq_lens,
+                       const int32_t* ref_counts, int32_t* page_table_out,
+                       int32_t* ref_counts_out, int32_t* num_used, size_t num_seqs,
+                       size_t max_pages, size_t num_pages, size_t page_size, void* workspace,
+                       hipStream_t stream);
+
+/* ---- 4-bit weights with a scale per group of columns (no counterpart in the
+ * reference): W[n][k] = (code[n][k] - 8) * scale[n][k / group_size], group_size a
+ * multiple of 32.  attn_w4_pack makes them from fp16 weights [out_dim][in_dim] (a
+ * layer's fused QKV weight, its o_proj, ...): scale = largest magnitude of the group /
+ * 7 rounded to fp16, code = W / scale rounded to nearest (ties to even) + 8.  packed:
+ * attn_w4_weight_bytes bytes, 16-byte aligned, codes in tiles of 16 rows x 128 columns;
+ * scales: attn_w4_scale_count fp16 values, [ceil(in_dim / group_size)][out_dim rounded up
+ * to 16].  Tile (i, j) is at (i * ceil(in_dim / 128) + j) * 1024 bytes: word 4 (16 a + r) +
+ * s holds row 16 i + r, columns 128 j + 32 s + 8 a + 0..7, column 2 e of the eight in bits
+ * 4 e and column 2 e + 1 in bits 16 + 4 e. */
+size_t attn_w4_weight_bytes(size_t out_dim, size_t in_dim);
+size_t attn_w4_scale_count(size_t out_dim, size_t in_dim, size_t group_size);
+int attn_w4_pack(const attn_f16_t* w, void* packed, attn_f16_t* scales, size_t out_dim,
+                 size_t in_dim, size_t group_size, hipStream_t stream);
+
+/* y[t] = W x[t] (+ residual[t]) for num_tokens tokens, fp16 in, fp32 accumulation, fp16
+ * out: attn_qkv_decode and attn_out_proj_decode (beta 1) on 4-bit weights, for one token
+ * or a batch.  x rows are x_stride apart, y and residual rows y_stride (0 = packed);
+ * residual may be y, or NULL.  in_dim == 0: y = residual, or zeros. */
+int attn_w4_matvec(const attn_f16_t* x, attn_f16_t* y, const void* packed,
+                   const attn_f16_t* scales, const attn_f16_t* residual, size_t num_tokens,
+                   size_t in_dim, size_t out_dim, size_t group_size, size_t x_stride,
+                   size_t y_stride, hipStream_t stream);
+
 /* Host-side RoPE tables, fp16 [max_seq_len][head_dim/2]: inv_freq[i] =
  * 1/powf(theta, 2i/D), angle = float(pos)*inv_freq[i], cos/sin in fp32 then
  * RNE to fp16.  Same tables as rope_cache.hpp:48-76 (create_rope_cache minus

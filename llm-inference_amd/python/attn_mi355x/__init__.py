@@ -94,6 +94,20 @@ def _declare(lib):
                                                _c.POINTER(WeightsLayout)]),
         "attn_weights_error_string": (_c.c_char_p, [_c.c_int]),
         "attn_graph_node_records": (_sz, []),
+        "attn_paged_rope_store_kv": (_c.c_int, [_vp] * 11 + [_sz] * 11 + [_c.c_int, _vp]),
+        "attn_paged_decode_workspace_bytes": (_sz, [_sz] * 4),
+        "attn_paged_decode": (_c.c_int, [_vp] * 6 + [_sz] * 8 + [_vp, _vp]),
+        "attn_pages_workspace_bytes": (_sz, [_sz, _sz]),
+        "attn_pages_copy": (_c.c_int, [_vp, _sz, _sz, _sz, _vp, _vp, _sz, _sz, _vp]),
+        "attn_pages_free": (_c.c_int, [_vp] * 4 + [_sz] * 4 + [_vp]),
+        "attn_pages_fork": (_c.c_int, [_vp] * 6 + [_sz] * 5 + [_vp]),
+        "attn_pages_grow": (_c.c_int, [_vp, _sz, _sz, _sz] + [_vp] * 5 + [_sz] * 4 + [_vp, _vp]),
+        "attn_pages_compact": (_c.c_int, [_vp, _sz, _sz, _sz] + [_vp] * 6 + [_sz] * 4 + [_vp,
+                                                                                        _vp]),
+        "attn_w4_weight_bytes": (_sz, [_sz, _sz]),
+        "attn_w4_scale_count": (_sz, [_sz, _sz, _sz]),
+        "attn_w4_pack": (_c.c_int, [_vp] * 3 + [_sz] * 3 + [_vp]),
+        "attn_w4_matvec": (_c.c_int, [_vp] * 5 + [_sz] * 6 + [_vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -123,7 +137,11 @@ def exported_symbols():
             "attn_update_rope_decode_nodes", "attn_weights_parse", "attn_weights_layout_for",
             "attn_decode_noalloc", "attn_out_proj_decode",
             "attn_decode_out_proj_workspace_bytes", "attn_decode_out_proj",
-            "attn_weights_error_string", "attn_graph_node_records"]
+            "attn_weights_error_string", "attn_graph_node_records",
+            "attn_paged_rope_store_kv", "attn_paged_decode_workspace_bytes", "attn_paged_decode",
+            "attn_pages_workspace_bytes", "attn_pages_copy", "attn_pages_free", "attn_pages_fork",
+            "attn_pages_grow", "attn_pages_compact", "attn_w4_weight_bytes",
+            "attn_w4_scale_count", "attn_w4_pack", "attn_w4_matvec"]
 
 
 def _ptr(x) -> Optional[int]:
@@ -298,6 +316,113 @@ def decode_out_proj(q, k_cache, v_cache, attn_out, partial_out, partial_max, par
         nodes[:] = [an.value, mn.value]
 
 
+def paged_rope_store_kv(q, k, v, k_pages, v_pages, cos, sin, page_table, positions, num_tokens,
+                        num_seqs, max_pages, num_pages, page_size, max_seq_len, num_heads,
+                        num_kv_heads, head_dim, q_stride=0, k_stride=0, apply_rotation=True,
+                        q_out=None, seq_ids=None, stream=None):
+    """rope_store_kv into the pages of a paged cache, for any set of tokens: token t
+    at positions[t] of sequence seq_ids[t] (None: sequence t)."""
+    rc = lib().attn_paged_rope_store_kv(
+        _ptr(q), _ptr(k), _ptr(v), _ptr(q_out), _ptr(k_pages), _ptr(v_pages), _ptr(cos),
+        _ptr(sin), _ptr(page_table), _ptr(seq_ids), _ptr(positions), num_tokens, num_seqs,
+        max_pages, num_pages, page_size, max_seq_len, num_heads, num_kv_heads, head_dim,
+        q_stride, k_stride, 1 if apply_rotation else 0, _stream(stream))
+    _check(rc, "attn_paged_rope_store_kv")
+
+
+def paged_decode_workspace(num_seqs, num_heads, num_kv_heads, head_dim, device="cuda"):
+    """The workspace paged_decode needs (contents do not matter)."""
+    n = int(lib().attn_paged_decode_workspace_bytes(num_seqs, num_heads, num_kv_heads, head_dim))
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def paged_decode(q, k_pages, v_pages, out, page_table, kv_lens, num_seqs, max_pages, num_pages,
+                 page_size, num_heads, num_kv_heads, head_dim, workspace, q_stride=0,
+                 stream=None):
+    """Decode attention of one new token per sequence over its pages."""
+    rc = lib().attn_paged_decode(_ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(out),
+                                 _ptr(page_table), _ptr(kv_lens), num_seqs, max_pages, num_pages,
+                                 page_size, num_heads, num_kv_heads, head_dim, q_stride,
+                                 _ptr(workspace), _stream(stream))
+    _check(rc, "attn_paged_decode")
+
+
+def pages_workspace(num_seqs, num_pages, device="cuda"):
+    """The workspace pages_grow and pages_compact need (contents do not matter)."""
+    n = int(lib().attn_pages_workspace_bytes(num_seqs, num_pages))
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def pages_copy(pool, num_planes, page_elems, src, dst, n, num_pages, plane_stride=0, stream=None):
+    """Pages src[i] -> dst[i] in every plane of the pool."""
+    rc = lib().attn_pages_copy(_ptr(pool), num_planes, plane_stride, page_elems, _ptr(src),
+                               _ptr(dst), n, num_pages, _stream(stream))
+    _check(rc, "attn_pages_copy")
+
+
+def pages_free(page_table, seq_lens, ref_counts, num_seqs, max_pages, num_pages, page_size,
+               keep_lens=None, stream=None):
+    """Cuts every sequence to keep_lens[b] tokens (None: 0)."""
+    rc = lib().attn_pages_free(_ptr(page_table), _ptr(seq_lens), _ptr(keep_lens),
+                               _ptr(ref_counts), num_seqs, max_pages, num_pages, page_size,
+                               _stream(stream))
+    _check(rc, "attn_pages_free")
+
+
+def pages_fork(src_table, src_lens, dst_table, dst_lens, parents, ref_counts, num_src, num_dst,
+               max_pages, num_pages, page_size, stream=None):
+    """Row i of the destination table shares the pages of source row parents[i]."""
+    rc = lib().attn_pages_fork(_ptr(src_table), _ptr(src_lens), _ptr(dst_table), _ptr(dst_lens),
+                               _ptr(parents), _ptr(ref_counts), num_src, num_dst, max_pages,
+                               num_pages, page_size, _stream(stream))
+    _check(rc, "attn_pages_fork")
+
+
+def pages_grow(pool, num_planes, page_elems, page_table, seq_lens, grow, ref_counts, status,
+               num_seqs, max_pages, num_pages, page_size, workspace, plane_stride=0,
+               stream=None):
+    """Sequence b grows by grow[b] tokens: new pages, and a copy of a shared last one."""
+    rc = lib().attn_pages_grow(_ptr(pool), num_planes, plane_stride, page_elems,
+                               _ptr(page_table), _ptr(seq_lens), _ptr(grow), _ptr(ref_counts),
+                               _ptr(status), num_seqs, max_pages, num_pages, page_size,
+                               _ptr(workspace), _stream(stream))
+    _check(rc, "attn_pages_grow")
+
+
+def pages_compact(pool, num_planes, page_elems, page_table, seq_lens, ref_counts, page_table_out,
+                  ref_counts_out, num_used, num_seqs, max_pages, num_pages, page_size, workspace,
+                  plane_stride=0, stream=None):
+    """Moves the used pages to the front of the pool."""
+    rc = lib().attn_pages_compact(_ptr(pool), num_planes, plane_stride, page_elems,
+                                  _ptr(page_table), _ptr(seq_lens), _ptr(ref_counts),
+                                  _ptr(page_table_out), _ptr(ref_counts_out), _ptr(num_used),
+                                  num_seqs, max_pages, num_pages, page_size, _ptr(workspace),
+                                  _stream(stream))
+    _check(rc, "attn_pages_compact")
+
+
+def w4_pack(w, out_dim, in_dim, group_size, stream=None):
+    """4-bit codes and group scales of fp16 weights [out_dim][in_dim] (a tensor, or a
+    view such as ModelWeights.qkv): (packed, scales) for w4_matvec."""
+    packed = torch.empty(int(lib().attn_w4_weight_bytes(out_dim, in_dim)), dtype=torch.uint8,
+                         device=w.device)
+    scales = torch.empty(int(lib().attn_w4_scale_count(out_dim, in_dim, group_size)),
+                         dtype=torch.float16, device=w.device)
+    rc = lib().attn_w4_pack(_ptr(w), _ptr(packed), _ptr(scales), out_dim, in_dim, group_size,
+                            _stream(stream))
+    _check(rc, "attn_w4_pack")
+    return packed, scales
+
+
+def w4_matvec(x, y, packed, scales, num_tokens, in_dim, out_dim, group_size, residual=None,
+              x_stride=0, y_stride=0, stream=None):
+    """y[t] = W x[t] (+ residual[t]) with 4-bit weights."""
+    rc = lib().attn_w4_matvec(_ptr(x), _ptr(y), _ptr(packed), _ptr(scales), _ptr(residual),
+                              num_tokens, in_dim, out_dim, group_size, x_stride, y_stride,
+                              _stream(stream))
+    _check(rc, "attn_w4_matvec")
+
+
 def decode_plan(kv_len, num_heads, num_kv_heads, head_dim, kv_stride=0, q=None, k=None,
                 v=None):
     out = (ctypes.c_uint32 * 5)()
@@ -359,6 +484,79 @@ class KVCache:
             raise IndexError(f"KV cache capacity exceeded: requested {n} tokens, capacity "
                              f"{self.max_seq_len}")
         self.cached_len = n
+
+
+class PagedKVCache:
+    """Paged KV cache of a batch of sequences: one pool for all layers with KVCache's
+    layout (max_seq_len = num_pages * page_size), page table, lengths and reference
+    counts on the device.  `status` holds what the last grow found missing (two int32:
+    pages the pool lacks, rows that are too short; then nothing has changed)."""
+
+    def __init__(self, num_layers, num_pages, page_size, num_kv_heads, head_dim, max_seqs,
+                 max_pages, device="cuda"):
+        self.num_layers, self.num_pages, self.page_size = num_layers, num_pages, page_size
+        self.num_kv_heads, self.head_dim = num_kv_heads, head_dim
+        self.max_seqs, self.max_pages = max_seqs, max_pages
+        self.page_elems = page_size * num_kv_heads * head_dim
+        self.pool = torch.empty(2 * num_layers, num_pages, self.page_elems, dtype=torch.float16,
+                                device=device)
+        self.page_table = torch.full((max_seqs, max_pages), -1, dtype=torch.int32, device=device)
+        self.seq_lens = torch.zeros(max_seqs, dtype=torch.int32, device=device)
+        self.ref_counts = torch.zeros(num_pages, dtype=torch.int32, device=device)
+        self.status = torch.zeros(2, dtype=torch.int32, device=device)
+        self.num_used = torch.zeros(1, dtype=torch.int32, device=device)
+        self._pages_ws = pages_workspace(max_seqs, num_pages, device)
+        self._decode_ws = {}
+
+    def k(self, layer):
+        return self.pool[2 * layer]
+
+    def v(self, layer):
+        return self.pool[2 * layer + 1]
+
+    def grow(self, tokens, stream=None):
+        """Each sequence by tokens[b] (int32 [max_seqs])."""
+        pages_grow(self.pool, 2 * self.num_layers, self.page_elems, self.page_table,
+                   self.seq_lens, tokens, self.ref_counts, self.status, self.max_seqs,
+                   self.max_pages, self.num_pages, self.page_size, self._pages_ws, stream=stream)
+
+    def free(self, keep_lens=None, stream=None):
+        """Each sequence cut to keep_lens[b] tokens (None: all to 0; -1: left alone)."""
+        pages_free(self.page_table, self.seq_lens, self.ref_counts, self.max_seqs,
+                   self.max_pages, self.num_pages, self.page_size, keep_lens, stream)
+
+    def fork(self, parents, stream=None):
+        """The empty sequence i becomes a fork of sequence parents[i] (-1: left alone)."""
+        pages_fork(self.page_table, self.seq_lens, self.page_table, self.seq_lens, parents,
+                   self.ref_counts, self.max_seqs, self.max_seqs, self.max_pages,
+                   self.num_pages, self.page_size, stream)
+
+    def compact(self, stream=None):
+        pages_compact(self.pool, 2 * self.num_layers, self.page_elems, self.page_table,
+                      self.seq_lens, self.ref_counts, self.page_table, self.ref_counts,
+                      self.num_used, self.max_seqs, self.max_pages, self.num_pages,
+                      self.page_size, self._pages_ws, stream=stream)
+
+    def append(self, layer, q, k, v, cos, sin, positions, num_tokens, num_heads, max_seq_len,
+               q_stride=0, k_stride=0, apply_rotation=True, q_out=None, seq_ids=None,
+               stream=None):
+        """paged_rope_store_kv into a layer's pages."""
+        paged_rope_store_kv(q, k, v, self.k(layer), self.v(layer), cos, sin, self.page_table,
+                            positions, num_tokens, self.max_seqs, self.max_pages,
+                            self.num_pages, self.page_size, max_seq_len, num_heads,
+                            self.num_kv_heads, self.head_dim, q_stride, k_stride,
+                            apply_rotation, q_out, seq_ids, stream)
+
+    def decode(self, layer, q, out, num_heads, q_stride=0, stream=None):
+        """paged_decode of one token per sequence over a layer's pages.  Calls on one
+        cache share a workspace and must be ordered."""
+        if num_heads not in self._decode_ws:
+            self._decode_ws[num_heads] = paged_decode_workspace(
+                self.max_seqs, num_heads, self.num_kv_heads, self.head_dim, self.pool.device)
+        paged_decode(q, self.k(layer), self.v(layer), out, self.page_table, self.seq_lens,
+                     self.max_seqs, self.max_pages, self.num_pages, self.page_size, num_heads,
+                     self.num_kv_heads, self.head_dim, self._decode_ws[num_heads], q_stride,
+                     stream)
 
 
 def _weights_error(rc: int, what: str):
