@@ -22,6 +22,7 @@ j * page and on.  4-bit weights lie in tiles of 16 rows and 128 columns, uint32
 8 a + 0..7 of the tile, column 2 i in bits 4 i and column 2 i + 1 in bits 16 + 4 i; a
 code c stands for (c - 8) * scale; scales are fp16 [column groups][rows padded to 16].
 """
+import functools
 import math
 import pathlib
 import random
@@ -44,6 +45,7 @@ VOCABULARY = 128256
 INTERMEDIATE = 11008
 
 
+@functools.cache
 def _binding():
     path = str(pathlib.Path.cwd() / "llm-inference_amd" / "python")
     if path not in sys.path:
