@@ -4,9 +4,37 @@
 //
 // A sequence of length 0 (a row of a padded batch) leaves its output as it was.  A
 // page number out of range makes its sequence's output NaN: nothing is read for it.
+//
+// Bound by the K/V bytes, 4 * Hkv * D per key; by latency for short contexts.
+//
+// Split.  The lengths are known on the device only, and differ.  The keys of all
+// sequences, in units of 32 keys and one after the other, make one line of units; each
+// workgroup of a KV head takes an equal, contiguous share of it (its position in the
+// line comes from a scan of the lengths that every wave does by itself).  So every
+// workgroup reads the same number of bytes whatever the lengths are, and the grid and
+// the workspace depend on neither batch nor lengths.  A share may hold the end of one
+// sequence, some whole ones and the start of another: whole ones are written to the
+// output at once, pieces to the workspace as fp32 states (running maximum, sum,
+// unnormalised output), and a second kernel joins a sequence's pieces.  Where no table
+// row can hold more than kWholeKeys keys, a workgroup per sequence and KV head and no
+// second kernel.
+//
+// A unit.  Four waves take units in turn, each with two in flight.  Scores are S^T = K
+// Q^T on v_mfma_f32_16x16x32_f16 (32 keys x up to 16 query heads of the KV head, so K and
+// V are read once for all of them; larger groups take further workgroups), with the key
+// rows ordered so that the result is the B operand of O^T = V^T P^T: lane (gq, n) holds
+// query n and keys 8 gq .. 8 gq + 7.  Pages enter through LDS: the workgroup turns its
+// part of the table into the pool row of every eight keys (of every key where the page
+// size is no multiple of 8), which a lane's loads start from.
+//
+// Rounding.  Scores, maxima, sums and states are fp32.  The weights are rounded to fp16
+// for the PV product, scaled by 2^15 (weights are at most 1): they keep 11 bits down to
+// 2^-29 of the largest, and the denominator sums the rounded ones.  V rows past the
+// sequence's end are set to zero in registers (the cache may hold anything there).
 #include "paged_internal.hpp"
 #include "../../include/attn_mi355x.h"
 
+#include <algorithm>
 #include <cmath>
 
 namespace attn {
@@ -32,8 +60,8 @@ struct PagedDecodeArgs {
     uint32_t pad_;
 };
 
-// Any head_dim up to 256, page size, alignment and grouping: one workgroup per
-// sequence and query head, tiles of 256 keys, one score per thread, then a dim per
+// Head dims other than 64 and 128, unaligned tensors: one workgroup per sequence and
+// query head, tiles of 256 keys, one score per thread, then a dim per
 // thread; fp32 throughout.
 constexpr int kTile = 256;
 
@@ -92,6 +120,466 @@ __global__ __launch_bounds__(kTile) void paged_decode_generic(PagedDecodeArgs a)
     if (tid < D) a.out[((uint64_t)b * a.num_heads + h) * D + tid] = (f16)(acc / l_run);
 }
 
+// ------------------------------------------------------------------ split and merge
+
+constexpr uint32_t kWaves = 4;
+constexpr uint32_t kThreads = 64 * kWaves;
+constexpr uint32_t kUnit = 32;          // keys
+constexpr uint32_t kMinUnits = 8;       // least share of a workgroup: two units a wave
+constexpr uint32_t kMaxGroups = 512;    // workgroups over all head groups (two per CU)
+constexpr uint32_t kWholeKeys = 384;    // longest table row that takes no split
+constexpr uint32_t kEntries = 1024;     // pool rows staged at once
+constexpr float kNoMax = -1.0e30f;      // finite: masked scores (-inf) get weight 0
+constexpr float kWeightBits = 15.0f;
+
+struct PagedSplitArgs {
+    PagedDecodeArgs d;
+    float* acc;           // [head groups][2 wgs][heads][D]  (workspace)
+    float* m;             // [head groups][2 wgs][heads], log2 domain
+    float* l;
+    uint32_t* plan;       // [num_seqs][2]: first and last workgroup of a sequence
+    uint32_t parts;       // head groups per KV head
+    uint32_t head_groups; // Hkv * parts
+    uint32_t heads;       // heads of a state: min(group, 16)
+    uint32_t wgs;         // workgroups per head group
+    uint32_t dim_parts;   // merge: workgroups per sequence and head
+};
+
+// v summed over the lanes up to this one: DPP row shifts within 16 lanes, then row
+// broadcasts
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, false);  // row_shr:1
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);  // row_bcast:15
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);  // row_bcast:31
+    return v;
+}
+
+__device__ __forceinline__ uint32_t units_of(const PagedDecodeArgs& a, uint32_t b) {
+    return b < a.num_seqs ? (clamp_len(a.lens[b], a.max_pages, a.page_size) + kUnit - 1u) / kUnit
+                          : 0u;
+}
+
+// A lane's reads of pool rows: BIG through 64-bit addresses; otherwise through a buffer
+// resource over the plane, whose 32-bit offsets take a multiply-add per row, and whose
+// reads of rows that are not live fetch nothing (an offset past the range).  Each byte
+// is read once per call: the non-temporal hint.
+template <bool BIG>
+struct PoolRows {
+    const char* base;
+    BufRsrc rsrc;
+    uint32_t row_bytes, lane_bytes;
+    __device__ PoolRows(const f16* plane, uint64_t bytes, uint32_t row, uint32_t lane)
+        : base(reinterpret_cast<const char*>(plane) + lane),
+          rsrc(make_rsrc(plane, (uint32_t)bytes)),
+          row_bytes(row),
+          lane_bytes(lane) {}
+    template <class T>
+    __device__ __forceinline__ T get(uint32_t row, uint32_t extra, bool live) const {
+        if constexpr (BIG) {
+            return __builtin_nontemporal_load(
+                reinterpret_cast<const T*>(base + (uint64_t)row * row_bytes + extra));
+        } else {
+            const uint32_t at = live ? row * row_bytes + lane_bytes : 0xfffff000u;
+            if constexpr (sizeof(T) == 16)
+                return __builtin_bit_cast(
+                    T, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)(at + extra), 0, 2));
+            else
+                return __builtin_bit_cast(
+                    T, __builtin_amdgcn_raw_buffer_load_b64(rsrc, (int)(at + extra), 0, 2));
+        }
+    }
+};
+
+// D: head dim (128 or 64).  OCT: the page size is a multiple of 8.  WHOLE: workgroup
+// (head group, sequence) takes the whole sequence.  BIG: a plane of 4 GiB or more.
+template <int D, bool OCT, bool WHOLE, bool BIG>
+__global__ __launch_bounds__(kThreads, 2) void paged_decode_split(PagedSplitArgs sa) {
+    constexpr int kSteps = D / 32;            // MFMAs of a score tile
+    constexpr int kTiles = D / 16;            // output tiles, dims {kTiles m + mt}
+    constexpr uint32_t kGran = OCT ? 8 : 1;   // keys per staged row
+    constexpr uint32_t kBlock = kEntries * kGran / kUnit;  // units staged at once
+    constexpr int kPitch = D + 4;
+    typedef _Float16 VRow __attribute__((ext_vector_type(kTiles)));
+    __shared__ uint32_t s_row[kEntries];
+    __shared__ __attribute__((aligned(16))) float s_acc[kWaves][16][kPitch];
+    __shared__ float s_m[kWaves][16], s_l[kWaves][16];
+    __shared__ uint32_t s_bad;
+    const PagedDecodeArgs& a = sa.d;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t n = lane & 15u, gq = lane >> 4;
+    const uint32_t hg = WHOLE ? blockIdx.x : blockIdx.x % sa.head_groups;
+    const uint32_t w = WHOLE ? 0u : blockIdx.x / sa.head_groups;
+    const uint32_t g = hg / sa.parts, part = hg - g * sa.parts;
+    const uint32_t h0 = g * a.group + 16u * part;
+    const uint32_t heads = min(16u, a.group - 16u * part);
+    const uint32_t row_bytes = a.num_kv_heads * D * 2u;
+    const uint64_t plane = (uint64_t)a.num_pages * a.page_size * row_bytes;
+    const PoolRows<BIG> rows_k(a.kp, plane, row_bytes, (g * D + 8u * gq) * 2u);
+    const PoolRows<BIG> rows_v(a.vp, plane, row_bytes, (g * D + (uint32_t)kTiles * n) * 2u);
+    struct Batch {
+        f16x8 k[2][kSteps];
+        VRow v[8];
+    };
+    // S^T row m of score tile tt is key 8 (m / 4) + 4 tt + m % 4 of the unit
+    const uint32_t koct = n >> 2, kin = n & 3u;
+
+    // this workgroup's units [u0, u1) of the line, the sequence that holds u0 and that
+    // sequence's first unit
+    uint32_t b, u, u1, base, share = 1;
+    if constexpr (WHOLE) {
+        b = blockIdx.y;
+        u = base = 0;
+        u1 = units_of(a, b);
+        if (u1 == 0) return;
+    } else {
+        uint32_t total = 0;
+        for (uint32_t b0 = 0; b0 < a.num_seqs; b0 += 64u)
+            total += (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(units_of(a, b0 + lane)), 63);
+        share = max(kMinUnits, (total + sa.wgs - 1u) / sa.wgs);
+        share = (share + kWaves - 1u) / kWaves * kWaves;  // the same number for each wave
+        if ((uint64_t)w * share >= total) return;
+        u = w * share;
+        u1 = min(total, u + share);
+        b = base = 0;
+        for (uint32_t b0 = 0;; b0 += 64u) {
+            const uint32_t mine = units_of(a, b0 + lane);
+            const uint32_t incl = wave_scan(mine);
+            const uint64_t past = __ballot(base + incl > u);
+            if (past) {
+                const int at = (int)__builtin_ctzll(past);
+                b = b0 + (uint32_t)at;
+                base += (uint32_t)__builtin_amdgcn_readlane((int)(incl - mine), at);
+                break;
+            }
+            base += (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
+        }
+    }
+
+    while (u < u1) {
+        const uint32_t len = clamp_len(a.lens[b], a.max_pages, a.page_size);
+        const uint32_t units = (len + kUnit - 1u) / kUnit;
+        if (units == 0) {
+            ++b;
+            continue;
+        }
+        const uint32_t rel = u - base;                    // first unit of this piece
+        const uint32_t count = min(units - rel, u1 - u);  // its units
+        const bool complete = count == units;
+
+        // Q^T as the B operand: lane (gq, n) holds Q[n][32 s + 8 gq ..]
+        f16x8 qb[kSteps];
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+            qb[s] = n < heads ? ld16(a.q + b * a.q_stride + (uint64_t)(h0 + n) * D + 32 * s + 8 * gq)
+                              : f16x8{};
+        f32x4 acc[kTiles];
+#pragma unroll
+        for (int mt = 0; mt < kTiles; ++mt) acc[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        float m_run = kNoMax, l_run = 0.f;
+        if (tid == 0) s_bad = 0;
+
+        for (uint32_t blk = 0; blk < count; blk += kBlock) {
+            const uint32_t nu = min(kBlock, count - blk);  // units of this block
+            const uint32_t key0 = (rel + blk) * kUnit;
+            __syncthreads();  // the last block's rows are read; s_bad is cleared
+            for (uint32_t i = tid; i < nu * (kUnit / kGran); i += kThreads) {
+                const uint32_t key = key0 + i * kGran;
+                uint32_t row = 0;
+                if (key < len) {
+                    const uint32_t j = key / a.page_size;
+                    const uint32_t page = (uint32_t)a.table[(uint64_t)b * a.max_pages + j];
+                    if (page < a.num_pages)
+                        row = page * a.page_size + (key - j * a.page_size);
+                    else
+                        s_bad = 1;
+                }
+                s_row[i] = row;
+            }
+            __syncthreads();
+            const uint32_t nk = min(len - key0, nu * kUnit);  // keys of this block
+
+            auto load = [&](uint32_t un, Batch& x) {
+                const bool live = un < nu;  // a load past the block fetches nothing of it
+#pragma unroll
+                for (int tt = 0; tt < 2; ++tt) {
+                    const uint32_t kr = OCT ? s_row[live ? 4u * un + koct : 0u] + 4u * tt + kin
+                                            : s_row[live ? 32u * un + 8u * koct + 4u * tt + kin : 0u];
+#pragma unroll
+                    for (int s = 0; s < kSteps; ++s)
+                        x.k[tt][s] = rows_k.template get<f16x8>(kr, 64u * s, live);
+                }
+#pragma unroll
+                for (uint32_t r = 0; r < 8; ++r) {
+                    const uint32_t vr = OCT ? s_row[live ? 4u * un + gq : 0u] + r
+                                            : s_row[live ? 32u * un + 8u * gq + r : 0u];
+                    x.v[r] = rows_v.template get<VRow>(vr, 0u, live);
+                }
+            };
+            auto compute = [&](uint32_t un, Batch& x) {
+                f32x4 st[2];
+#pragma unroll
+                for (int tt = 0; tt < 2; ++tt) {
+                    st[tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int s = 0; s < kSteps; ++s) st[tt] = mfma16(x.k[tt][s], qb[s], st[tt]);
+                }
+                if ((un + 1u) * kUnit > nk) {  // the unit that holds the sequence's end
+                    const uint32_t left = nk - un * kUnit;
+#pragma unroll
+                    for (uint32_t r = 0; r < 8; ++r)
+                        if (8u * gq + r >= left) {
+                            st[r >> 2][r & 3] = -INFINITY;
+                            x.v[r] = VRow{};
+                        }
+                }
+                float mx = st[0][0];
+#pragma unroll
+                for (int r = 1; r < 8; ++r) mx = fmaxf(mx, st[r >> 2][r & 3]);
+                mx = max_xor<32>(max_xor<16>(mx)) * a.scale_log2;
+                const float m_new = fmaxf(m_run, mx);
+                const float alpha = fast_exp2(m_run - m_new);
+                const float shift = kWeightBits - m_new;
+                f16x8 p;
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    p[r] = (f16)fast_exp2(__builtin_fmaf(st[r >> 2][r & 3], a.scale_log2, shift));
+                const f16x2 one = {(f16)1.0f, (f16)1.0f};
+                float sum = 0.f;
+#pragma unroll
+                for (int r = 0; r < 8; r += 2)
+                    sum = __builtin_amdgcn_fdot2(f16x2{p[r], p[r + 1]}, one, sum, false);
+                l_run = l_run * alpha + sum;
+                m_run = m_new;
+#pragma unroll
+                for (int mt = 0; mt < kTiles; ++mt) {
+                    f16x8 va;
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) va[r] = x.v[r][mt];
+                    acc[mt] = mfma16(va, p, acc[mt] * alpha);
+                }
+            };
+
+            // Units wave, wave + 4, ...; two in flight, the next load going out as soon as
+            // a unit is computed.  Every path into the loop has exactly A and B in flight,
+            // so that the compiler's wait for A leaves B's loads running; the scheduler
+            // barriers keep the loads of one unit out of the arithmetic of another (without
+            // them the 128-dim kernels spilled 128 registers).
+            // Planes of 4 GiB or more take one unit at a time (two and their 64-bit addresses do
+            // not fit the registers).
+            uint32_t un = wave;
+            Batch A, B;
+            if constexpr (BIG) {
+                for (; un < nu; un += kWaves) {
+                    load(un, A);
+                    compute(un, A);
+                }
+            } else if (un + kWaves < nu) {
+                load(un, A);
+                load(un + kWaves, B);
+                while (un + 2u * kWaves < nu) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    compute(un, A);
+                    load(un + 2u * kWaves, A);
+                    __builtin_amdgcn_sched_barrier(0);
+                    compute(un + kWaves, B);
+                    load(un + 3u * kWaves, B);
+                    un += 2u * kWaves;
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                compute(un, A);
+                __builtin_amdgcn_sched_barrier(0);
+                if (un + kWaves < nu) compute(un + kWaves, B);
+            } else if (un < nu) {
+                load(un, A);
+                compute(un, A);
+            }
+        }
+
+        // the waves' states meet in LDS
+        l_run = add_xor<32>(add_xor<16>(l_run));
+        if (n < heads) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int t4 = 0; t4 < kTiles; t4 += 4)
+                    *reinterpret_cast<f32x4*>(&s_acc[wave][n][kTiles * (4 * gq + i) + t4]) =
+                        f32x4{acc[t4][i], acc[t4 + 1][i], acc[t4 + 2][i], acc[t4 + 3][i]};
+        }
+        if (gq == 0) {
+            s_m[wave][n] = m_run;
+            s_l[wave][n] = l_run;
+        }
+        __syncthreads();
+        const uint64_t slot = WHOLE ? 0 : (uint64_t)hg * 2u * sa.wgs + 2u * w + (rel == 0 ? 1u : 0u);
+        for (uint32_t i = tid; i < heads * (D / 4); i += kThreads) {
+            const uint32_t h = i / (D / 4), d = 4u * (i - h * (D / 4));
+            float M = s_m[0][h];
+#pragma unroll
+            for (uint32_t x = 1; x < kWaves; ++x) M = fmaxf(M, s_m[x][h]);
+            f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+            float L = 0.f;
+#pragma unroll
+            for (uint32_t x = 0; x < kWaves; ++x) {
+                const float wt = fast_exp2(s_m[x][h] - M);
+                sum += *reinterpret_cast<const f32x4*>(&s_acc[x][h][d]) * wt;
+                L += s_l[x][h] * wt;
+            }
+            if (s_bad) L = __builtin_nanf("");
+            if (complete) {
+                const float inv = 1.0f / L;
+                const f16x4 o = {(f16)(sum[0] * inv), (f16)(sum[1] * inv), (f16)(sum[2] * inv),
+                                 (f16)(sum[3] * inv)};
+                *reinterpret_cast<f16x4*>(a.out + ((uint64_t)b * a.num_heads + h0 + h) * D + d) = o;
+            } else if constexpr (!WHOLE) {
+                const uint64_t st = slot * sa.heads + h;
+                *reinterpret_cast<f32x4*>(sa.acc + st * D + d) = sum;
+                if (d == 0) {
+                    sa.m[st] = M;
+                    sa.l[st] = L;
+                }
+            }
+        }
+        if constexpr (!WHOLE) {
+            if (rel == 0 && hg == 0 && tid == 0) {
+                sa.plan[2 * b] = w;
+                sa.plan[2 * b + 1] = (base + units - 1u) / share;
+            }
+        }
+        __syncthreads();  // the states are read
+        u += count;
+        base += units;
+        ++b;
+    }
+}
+
+// Joins the pieces of sequence blockIdx.y for one query head (for a part of its dims):
+// weights of the pieces' maxima, then 4 dims a thread, the pieces shared out over the
+// thread groups.  A sequence in one piece is written already.
+template <int D>
+__global__ __launch_bounds__(kThreads) void paged_decode_merge(PagedSplitArgs sa) {
+    __shared__ float s_w[kMaxGroups], s_red[2][kWaves];
+    __shared__ __attribute__((aligned(16))) f32x4 s_x[kThreads];
+    const PagedDecodeArgs& a = sa.d;
+    const uint32_t b = blockIdx.y, tid = threadIdx.x, wave = tid >> 6;
+    const uint32_t h = blockIdx.x / sa.dim_parts, dp = blockIdx.x - h * sa.dim_parts;
+    if (units_of(a, b) == 0) return;
+    const uint32_t wf = sa.plan[2 * b], pieces = sa.plan[2 * b + 1] - wf + 1u;
+    if (pieces == 1) return;
+    const uint32_t g = h / a.group, in_group = h - g * a.group;
+    const uint32_t hg = g * sa.parts + in_group / 16u;
+    const uint64_t hg0 = (uint64_t)hg * 2u * sa.wgs;
+    // state of piece j: the first one begins its sequence within its workgroup's share
+    auto state = [&](uint32_t j) {
+        return (hg0 + 2u * (wf + j) + (j == 0 ? 1u : 0u)) * sa.heads + in_group % 16u;
+    };
+    const uint32_t lanes = D / 4 / sa.dim_parts, groups = kThreads / lanes;
+    const uint32_t grp = tid / lanes, d = dp * (D / sa.dim_parts) + 4u * (tid - grp * lanes);
+    // the first pieces of each thread, alongside the maxima
+    constexpr uint32_t kFirst = 4;
+    f32x4 x0[kFirst];
+#pragma unroll
+    for (uint32_t i = 0; i < kFirst; ++i) {
+        const uint32_t j = grp + groups * i;
+        x0[i] = j < pieces ? *reinterpret_cast<const f32x4*>(sa.acc + state(j) * D + d)
+                           : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    static_assert(kMaxGroups == 2 * kThreads);
+    float m[2], l[2];
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i) {
+        const uint32_t j = tid + i * kThreads;
+        m[i] = j < pieces ? sa.m[state(j)] : -INFINITY;
+        l[i] = j < pieces ? sa.l[state(j)] : 0.f;
+    }
+    const float wm = wave_max(fmaxf(m[0], m[1]));
+    if ((tid & 63u) == 0) s_red[0][wave] = wm;
+    __syncthreads();
+    const float M = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
+    float den = 0.f;
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i) {
+        const float wt = fast_exp2(m[i] - M);
+        s_w[tid + i * kThreads] = wt;
+        if (tid + i * kThreads < pieces) den += wt * l[i];
+    }
+    den = wave_sum(den);
+    if ((tid & 63u) == 0) s_red[1][wave] = den;
+    __syncthreads();
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (uint32_t i = 0; i < kFirst; ++i) {
+        const uint32_t j = grp + groups * i;
+        if (j < pieces) x += x0[i] * s_w[j];
+    }
+#pragma unroll 4
+    for (uint32_t j = grp + groups * kFirst; j < pieces; j += groups)
+        x += *reinterpret_cast<const f32x4*>(sa.acc + state(j) * D + d) * s_w[j];
+    s_x[tid] = x;
+    __syncthreads();
+    if (grp != 0) return;
+    for (uint32_t i = 1; i < groups; ++i) x += s_x[tid + i * lanes];
+    const float inv = 1.0f / ((s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]));
+    const f16x4 o = {(f16)(x[0] * inv), (f16)(x[1] * inv), (f16)(x[2] * inv), (f16)(x[3] * inv)};
+    *reinterpret_cast<f16x4*>(a.out + ((uint64_t)b * a.num_heads + h) * D + d) = o;
+}
+
+// ------------------------------------------------------------------ host side
+
+// Sizes of the split plan, and the workspace's arrays as byte offsets
+struct PagedPlan {
+    uint32_t parts, head_groups, heads, wgs;
+    uint64_t at_m, at_l, at_acc, bytes;
+};
+
+PagedPlan paged_plan(size_t num_seqs, size_t num_heads, size_t num_kv_heads, size_t head_dim) {
+    PagedPlan p{};
+    const size_t group = num_heads / num_kv_heads;
+    p.parts = (uint32_t)((group + 15) / 16);
+    p.head_groups = (uint32_t)num_kv_heads * p.parts;
+    p.heads = (uint32_t)std::min<size_t>(group, 16);
+    p.wgs = std::max(1u, kMaxGroups / p.head_groups);
+    const uint64_t states = 2ull * p.head_groups * p.wgs * p.heads;
+    p.at_m = (num_seqs * 8 + 15) / 16 * 16;
+    p.at_l = p.at_m + (states * 4 + 15) / 16 * 16;
+    p.at_acc = p.at_l + (states * 4 + 15) / 16 * 16;
+    p.bytes = p.at_acc + states * head_dim * 4;
+    return p;
+}
+
+bool paged_split_dim(size_t head_dim) { return head_dim == 128 || head_dim == 64; }
+
+template <int D, bool OCT, bool BIG>
+hipError_t launch_split(const PagedSplitArgs& a, bool whole, hipStream_t stream) {
+    if (whole) {
+        hipLaunchKernelGGL((paged_decode_split<D, OCT, true, BIG>),
+                           dim3(a.head_groups, a.d.num_seqs), dim3(kThreads), 0, stream, a);
+        return hipGetLastError();
+    }
+    hipLaunchKernelGGL((paged_decode_split<D, OCT, false, BIG>), dim3(a.head_groups * a.wgs),
+                       dim3(kThreads), 0, stream, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((paged_decode_merge<D>), dim3(a.d.num_heads * a.dim_parts, a.d.num_seqs),
+                       dim3(kThreads), 0, stream, a);
+    return hipGetLastError();
+}
+
+template <int D>
+hipError_t launch_split(const PagedSplitArgs& a, bool whole, hipStream_t stream) {
+    // buffer offsets reach 0xffffefff; the ones past it stand for rows that are not read
+    const bool big = (uint64_t)a.d.num_pages * a.d.page_size * a.d.num_kv_heads * D * 2 > 0xffffe000ull;
+    const bool oct = a.d.page_size % 8 == 0;
+    if (big)
+        return oct ? launch_split<D, true, true>(a, whole, stream)
+                   : launch_split<D, false, true>(a, whole, stream);
+    return oct ? launch_split<D, true, false>(a, whole, stream)
+               : launch_split<D, false, false>(a, whole, stream);
+}
+
 }  // namespace
 }  // namespace attn
 
@@ -101,8 +589,8 @@ extern "C" {
 
 size_t attn_paged_decode_workspace_bytes(size_t num_seqs, size_t num_heads, size_t num_kv_heads,
                                          size_t head_dim) {
-    (void)num_seqs; (void)num_heads; (void)num_kv_heads; (void)head_dim;
-    return 256;
+    if (!paged_split_dim(head_dim) || num_kv_heads == 0 || num_heads < num_kv_heads) return 16;
+    return paged_plan(num_seqs, num_heads, num_kv_heads, head_dim).bytes;
 }
 
 int attn_paged_decode(const attn_f16_t* q, const attn_f16_t* k_pages, const attn_f16_t* v_pages,
@@ -114,7 +602,7 @@ int attn_paged_decode(const attn_f16_t* q, const attn_f16_t* k_pages, const attn
     if (!paged_sizes_ok(num_seqs, max_pages, num_pages, page_size) || num_kv_heads == 0 ||
         num_heads % num_kv_heads != 0 || num_heads > 65535 || num_seqs > 65535 || head_dim == 0 ||
         head_dim > 256 || !q || !k_pages || !v_pages || !out || !page_table || !kv_lens ||
-        !workspace)
+        !workspace || !aligned16(workspace))
         return (int)hipErrorInvalidValue;
     PagedDecodeArgs a{};
     a.q = reinterpret_cast<const f16*>(q);
@@ -133,6 +621,29 @@ int attn_paged_decode(const attn_f16_t* q, const attn_f16_t* k_pages, const attn
     a.group = (uint32_t)(num_heads / num_kv_heads);
     a.head_dim = (uint32_t)head_dim;
     a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)head_dim));
+    const uint64_t row_units = (max_pages * page_size + kUnit - 1) / kUnit;
+    if (paged_split_dim(head_dim) && num_pages > 0 && a.q_stride % 8 == 0 && aligned16(q) &&
+        aligned16(k_pages) && aligned16(v_pages) && aligned16(out) &&
+        paged_mul(num_seqs, row_units) <= 0x7fffffffull &&
+        get_option(kOptDecodeForceGeneric) == 0) {
+        const PagedPlan p = paged_plan(num_seqs, num_heads, num_kv_heads, head_dim);
+        PagedSplitArgs sa{};
+        sa.d = a;
+        char* const ws = static_cast<char*>(workspace);
+        sa.plan = reinterpret_cast<uint32_t*>(ws);
+        sa.m = reinterpret_cast<float*>(ws + p.at_m);
+        sa.l = reinterpret_cast<float*>(ws + p.at_l);
+        sa.acc = reinterpret_cast<float*>(ws + p.at_acc);
+        sa.parts = p.parts;
+        sa.head_groups = p.head_groups;
+        sa.heads = p.heads;
+        sa.wgs = p.wgs;
+        // few sequences: more workgroups of fewer dims each join a long one's pieces
+        sa.dim_parts = num_seqs * num_heads < 128 ? 4u : 1u;
+        const bool whole = max_pages * page_size <= kWholeKeys;
+        return (int)(head_dim == 128 ? launch_split<128>(sa, whole, stream)
+                                     : launch_split<64>(sa, whole, stream));
+    }
     hipLaunchKernelGGL(paged_decode_generic, dim3(a.num_heads, a.num_seqs), dim3(kTile), 0, stream,
                        a);
     return (int)hipGetLastError();
