@@ -386,11 +386,11 @@ int attn_pages_compact(attn_f16_t* pool, size_t num_planes, size_t plane_stride,
 
 /* ---- 4-bit weights with a scale per group of columns (no counterpart in the
  * reference): W[n][k] = (code[n][k] - 8) * scale[n][k / group_size], group_size a
- * multiple of 32.  attn_w4_pack makes them from fp16 weights [out_dim][in_dim] (a
+ * multiple of 32, in_dim at most 2^20.  attn_w4_pack makes them from fp16 weights [out_dim][in_dim] (a
  * layer's fused QKV weight, its o_proj, ...): scale = largest magnitude of the group /
  * 7 rounded to fp16, code = W / scale rounded to nearest (ties to even) + 8.  packed:
  * attn_w4_weight_bytes bytes, 16-byte aligned, codes in tiles of 16 rows x 128 columns;
- * scales: attn_w4_scale_count fp16 values, [ceil(in_dim / group_size)][out_dim rounded up
+ * scales (8-byte aligned): attn_w4_scale_count fp16 values, [ceil(in_dim / group_size)][out_dim rounded up
  * to 16].  Tile (i, j) is at (i * ceil(in_dim / 128) + j) * 1024 bytes: word 4 (16 a + r) +
  * s holds row 16 i + r, columns 128 j + 32 s + 8 a + 0..7, column 2 e of the eight in bits
  * 4 e and column 2 e + 1 in bits 16 + 4 e. */

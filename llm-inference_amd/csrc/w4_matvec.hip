@@ -15,6 +15,8 @@
 #include "attn_internal.hpp"
 #include "../../include/attn_mi355x.h"
 
+#include <algorithm>
+
 namespace attn {
 namespace {
 
@@ -30,8 +32,10 @@ struct W4Args {
     uint32_t rows;
     uint32_t cols;
     uint32_t group;
+    uint32_t group_mul;    // see w4_group
     uint32_t row_tiles;    // ceil(rows / 16)
     uint32_t col_tiles;    // ceil(cols / 128)
+    uint32_t split;        // waves that share a row tile: 1, 2, 4 or 8
 };
 
 // The eight columns of a word as fp16, in order: 1024 + code has the code in its lowest
@@ -48,83 +52,186 @@ __device__ __forceinline__ f16x8 w4_values(uint32_t word) {
     return v;
 }
 
-// Eight columns of x from k on, zero from `cols` on.  VEC: 16-byte loads (rows 16-byte
-// aligned, cols a multiple of 8).
-template <bool VEC>
-__device__ __forceinline__ f16x8 w4_load_x(const f16* row, uint32_t k, uint32_t cols) {
-    f16x8 v = {};
-    if constexpr (VEC) {
-        if (k < cols) v = ld16(row + k);
-    } else {
-#pragma unroll
-        for (uint32_t e = 0; e < 8; ++e)
-            if (k + e < cols) v[e] = row[k + e];
-    }
-    return v;
+constexpr uint32_t kW4Waves = 8;
+constexpr uint32_t kDead = 0xfffff000u;  // a buffer offset past every range: nothing is read
+
+// index of the scale of column k: k / group.  group_mul is 2^31 over the group in steps of
+// 32 columns, rounded up (0: one group): exact while steps times steps of a group stay
+// below 2^31, as they do up to 2^20 columns.
+__device__ __forceinline__ uint32_t w4_group(const W4Args& a, uint32_t k) {
+    return __umulhi(k >> 5 << 1, a.group_mul);
 }
 
-constexpr uint32_t kW4Waves = 8;
+// Sums of the waves that share a row tile: `part` waves (a power of two) of the workgroup's
+// eight, wave-contiguous.  s_part is [wave][tokens][17].
+template <int TOKENS>
+__device__ __forceinline__ void w4_store(const W4Args& a, const float (*s_part)[TOKENS][17],
+                                         uint32_t t0, uint32_t live) {
+    const uint32_t tiles = kW4Waves / a.split, first = blockIdx.x * tiles;
+    const uint32_t per_tile = live * 16u;
+    for (uint32_t i = threadIdx.x; i < tiles * per_tile; i += 64u * kW4Waves) {
+        const uint32_t tile = i / per_tile, j = i - tile * per_tile;
+        const uint32_t t = j >> 4, r = j & 15u, row = (first + tile) * 16u + r;
+        if (row >= a.rows) continue;
+        float sum = 0.f;
+        for (uint32_t x = 0; x < a.split; ++x) sum += s_part[tile * a.split + x][t][r];
+        const uint64_t at = (uint64_t)(t0 + t) * a.y_stride + row;
+        if (a.residual) sum += (float)a.residual[at];
+        a.y[at] = (f16)sum;
+    }
+}
 
-// One workgroup per 16 rows; its waves take the column tiles in turn and meet in LDS.
-// TT: tiles of 16 tokens.  SPS: steps of 32 columns that share a scale at least (4: the
-// group is a multiple of 128; 2: of 64; 1).  The products of a scale's columns are summed
-// by the MFMAs from zero, then scaled and added in fp32, so no product is rounded.
+// Up to four tokens.  Column n of the MFMAs' result stands for token n / 4 and step n % 4
+// of a column tile: lane (gq, n) loads x for that step only (one load per column tile
+// instead of four), the operand of step s is zero in the other steps' columns, and each
+// lane scales its column's sum by its own step's scales, whatever the group size.
+template <bool VEC>
+__global__ __launch_bounds__(64 * kW4Waves) void w4_matvec_narrow(W4Args a) {
+    constexpr int kDepth = 4;  // column tiles in flight
+    __shared__ float s_part[kW4Waves][4][17];
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t n = lane & 15u, gq = lane >> 4, step = n & 3u;
+    const uint32_t rt = (blockIdx.x * kW4Waves + wave) / a.split;
+    const uint32_t first = wave & (a.split - 1u);
+    const uint32_t token = min(n >> 2, a.tokens - 1u);
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    if (rt < a.row_tiles && a.col_tiles > 0) {
+        const BufRsrc rw =
+            make_rsrc(a.w + (uint64_t)rt * a.col_tiles * 256u, a.col_tiles * 1024u);
+        const f16* const xr = a.x + token * a.x_stride;
+        const BufRsrc rx = make_rsrc(a.x, (uint32_t)(((a.tokens - 1u) * a.x_stride + a.cols) * 2u));
+        const uint32_t x_at = (uint32_t)(token * a.x_stride) * 2u;
+        const f16* const sc = a.scales + rt * 16u + 4u * gq;
+        const uint64_t sc_stride = (uint64_t)a.row_tiles * 16u;
+        struct Stage {
+            u32x4 w;
+            f16x8 x;
+            f16x4 scale;
+        } st[kDepth];
+        auto load = [&](uint32_t c, Stage& z) {
+            z.w = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                rw, (int)(c * 1024u + 16u * lane), 0, 2));
+            const uint32_t k = 128u * c + 32u * step + 8u * gq;
+            if constexpr (VEC) {
+                z.x = buf_ld16(rx, k < a.cols ? x_at + 2u * k : kDead);
+            } else {
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e) z.x[e] = k + e < a.cols ? xr[k + e] : (f16)0.f;
+            }
+            z.scale = *reinterpret_cast<const f16x4*>(
+                sc + w4_group(a, min(128u * c + 32u * step, a.cols - 1u)) * sc_stride);
+        };
+#pragma unroll
+        for (int i = 0; i < kDepth; ++i) load(first + i * a.split, st[i]);
+        for (uint32_t c = first; c < a.col_tiles; c += kDepth * a.split) {
+#pragma unroll
+            for (int i = 0; i < kDepth; ++i) {
+                __builtin_amdgcn_sched_barrier(0);
+                if (c + i * a.split < a.col_tiles) {
+                    f32x4 part = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (uint32_t s = 0; s < 4; ++s)
+                        part = mfma16(w4_values(st[i].w[s]), step == s ? st[i].x : f16x8{}, part);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        acc[r] = __builtin_fmaf((float)st[i].scale[r], part[r], acc[r]);
+                }
+                load(c + (i + kDepth) * a.split, st[i]);
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {  // the four steps of a token
+        float v = acc[r];
+        v += dpp_f<kDppXor1>(v);
+        v += dpp_f<kDppXor2>(v);
+        if (step == 0) s_part[wave][n >> 2][4u * gq + r] = v;
+    }
+    __syncthreads();
+    w4_store<4>(a, s_part, 0, a.tokens);
+}
+
+// Any number of tokens, TT tiles of 16 at a time.  SPS: steps of 32 columns that share a
+// scale at least (4: the group is a multiple of 128; 2: of 64; 1).  The products of a
+// scale's columns are summed by the MFMAs from zero, then scaled and added in fp32, so no
+// product is rounded.
 template <int TT, int SPS, bool VEC>
 __global__ __launch_bounds__(64 * kW4Waves) void w4_matvec(W4Args a) {
-    constexpr int kRound = 4;  // column tiles in flight
+    constexpr int kDepth = TT == 1 ? 4 : 2;  // column tiles in flight
     __shared__ float s_part[kW4Waves][16 * TT][17];
-    const uint32_t tid = threadIdx.x, lane = tid & 63u;
-    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t n = lane & 15u, gq = lane >> 4;
-    const uint32_t rt = blockIdx.x, t0 = blockIdx.y * 16u * TT;
+    const uint32_t rt = (blockIdx.x * kW4Waves + wave) / a.split;
+    const uint32_t first = wave & (a.split - 1u);
+    const uint32_t t0 = blockIdx.y * 16u * TT;
     const uint32_t live = min(a.tokens - t0, 16u * (uint32_t)TT);
-    const uint64_t tile_words = (uint64_t)a.col_tiles * 256u;
-    const BufRsrc rw = make_rsrc(a.w + rt * tile_words, a.col_tiles * 1024u);
-    const f16* xr[TT];
-#pragma unroll
-    for (int tt = 0; tt < TT; ++tt)  // lanes past the last token repeat it; nothing of theirs is stored
-        xr[tt] = a.x + (uint64_t)(t0 + min(16u * tt + n, live - 1u)) * a.x_stride + 8u * gq;
-    const f16* const sc = a.scales + rt * 16u + 4u * gq;
-    const uint64_t sc_stride = (uint64_t)a.row_tiles * 16u;
-
     f32x4 acc[TT];
 #pragma unroll
     for (int tt = 0; tt < TT; ++tt) acc[tt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (uint32_t c0 = wave; c0 < a.col_tiles; c0 += kRound * kW4Waves) {
-        u32x4 w[kRound];
+    if (rt < a.row_tiles && a.col_tiles > 0) {
+        const BufRsrc rw =
+            make_rsrc(a.w + (uint64_t)rt * a.col_tiles * 256u, a.col_tiles * 1024u);
+        const f16* const xb = a.x + (uint64_t)t0 * a.x_stride;
+        const BufRsrc rx = make_rsrc(xb, (uint32_t)(((live - 1u) * a.x_stride + a.cols) * 2u));
+        uint64_t x_at[TT];  // elements
 #pragma unroll
-        for (int i = 0; i < kRound; ++i)  // past the last tile: nothing is read
-            w[i] = __builtin_bit_cast(
-                u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                           rw, (int)((c0 + i * kW4Waves) * 1024u + 16u * lane), 0, 2));
+        for (int tt = 0; tt < TT; ++tt)  // lanes past the last token repeat it; nothing of theirs is stored
+            x_at[tt] = min(16u * tt + n, live - 1u) * a.x_stride;
+        const f16* const sc = a.scales + rt * 16u + 4u * gq;
+        const uint64_t sc_stride = (uint64_t)a.row_tiles * 16u;
+        struct Stage {
+            u32x4 w;
+            f16x8 x[4][TT];
+            f16x4 scale[4 / SPS];
+        } st[kDepth];
+        auto load = [&](uint32_t c, Stage& z) {
+            z.w = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                rw, (int)(c * 1024u + 16u * lane), 0, 2));
 #pragma unroll
-        for (int i = 0; i < kRound; ++i) {
-            const uint32_t c = c0 + i * kW4Waves;
-            if (c >= a.col_tiles) break;
+            for (int s = 0; s < 4; ++s) {
+                const uint32_t k = 128u * c + 32u * s + 8u * gq;
+                if (s % SPS == 0)
+                    z.scale[s / SPS] = *reinterpret_cast<const f16x4*>(
+                        sc + w4_group(a, min(128u * c + 32u * s, a.cols - 1u)) * sc_stride);
 #pragma unroll
-            for (int s0 = 0; s0 < 4; s0 += SPS) {
-                const uint32_t k = 128u * c + 32u * s0;
-                if (SPS < 4 && k >= a.cols) break;
-                f32x4 part[TT];
+                for (int tt = 0; tt < TT; ++tt) {
+                    if constexpr (VEC) {
+                        z.x[s][tt] =
+                            buf_ld16(rx, k < a.cols ? 2u * ((uint32_t)x_at[tt] + k) : kDead);
+                    } else {
 #pragma unroll
-                for (int tt = 0; tt < TT; ++tt) part[tt] = f32x4{0.f, 0.f, 0.f, 0.f};
-                const f16x4 scale = *reinterpret_cast<const f16x4*>(sc + k / a.group * sc_stride);
-#pragma unroll
-                for (int s = s0; s < s0 + SPS; ++s) {
-                    const f16x8 wv = w4_values(w[i][s]);
-#pragma unroll
-                    for (int tt = 0; tt < TT; ++tt) {
-                        // x's rows start at column 8 gq
-                        const f16x8 xv = w4_load_x<VEC>(xr[tt], 128u * c + 32u * s,
-                                                        a.cols > 8u * gq ? a.cols - 8u * gq : 0u);
-                        part[tt] = mfma16(wv, xv, part[tt]);
+                        for (uint32_t e = 0; e < 8; ++e)
+                            z.x[s][tt][e] = k + e < a.cols ? xb[x_at[tt] + k + e] : (f16)0.f;
                     }
                 }
+            }
+        };
 #pragma unroll
-                for (int tt = 0; tt < TT; ++tt)
+        for (int i = 0; i < kDepth; ++i) load(first + i * a.split, st[i]);
+        for (uint32_t c = first; c < a.col_tiles; c += kDepth * a.split) {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        acc[tt][r] = __builtin_fmaf((float)scale[r], part[tt][r], acc[tt][r]);
+            for (int i = 0; i < kDepth; ++i) {
+                __builtin_amdgcn_sched_barrier(0);
+                if (c + i * a.split < a.col_tiles) {
+                    f32x4 part[TT];
+#pragma unroll
+                    for (int s = 0; s < 4; ++s) {
+                        const f16x8 wv = w4_values(st[i].w[s]);
+#pragma unroll
+                        for (int tt = 0; tt < TT; ++tt) {
+                            if (s % SPS == 0) part[tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+                            part[tt] = mfma16(wv, st[i].x[s][tt], part[tt]);
+                            if (s % SPS == SPS - 1)
+#pragma unroll
+                                for (int r = 0; r < 4; ++r)
+                                    acc[tt][r] = __builtin_fmaf((float)st[i].scale[s / SPS][r],
+                                                                part[tt][r], acc[tt][r]);
+                        }
+                    }
+                }
+                load(c + (i + kDepth) * a.split, st[i]);
             }
         }
     }
@@ -133,25 +240,17 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matvec(W4Args a) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) s_part[wave][16 * tt + n][4u * gq + r] = acc[tt][r];
     __syncthreads();
-    for (uint32_t i = tid; i < live * 16u; i += 64u * kW4Waves) {
-        const uint32_t t = i >> 4, r = i & 15u, row = rt * 16u + r;
-        if (row >= a.rows) continue;
-        float sum = 0.f;
-#pragma unroll
-        for (uint32_t x = 0; x < kW4Waves; ++x) sum += s_part[x][t][r];
-        const uint64_t at = (uint64_t)(t0 + t) * a.y_stride + row;
-        if (a.residual) sum += (float)a.residual[at];
-        a.y[at] = (f16)sum;
-    }
+    w4_store<16 * TT>(a, s_part, t0, live);
 }
 
 template <int TT, int SPS>
 hipError_t launch_w4(const W4Args& a, bool vec, hipStream_t stream) {
-    const dim3 grid(a.row_tiles, (a.tokens + 16u * TT - 1u) / (16u * TT)), block(64 * kW4Waves);
+    const uint32_t tiles = kW4Waves / a.split;
+    const dim3 grid((a.row_tiles + tiles - 1u) / tiles, (a.tokens + 16u * TT - 1u) / (16u * TT));
     if (vec)
-        hipLaunchKernelGGL((w4_matvec<TT, SPS, true>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((w4_matvec<TT, SPS, true>), grid, dim3(64 * kW4Waves), 0, stream, a);
     else
-        hipLaunchKernelGGL((w4_matvec<TT, SPS, false>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((w4_matvec<TT, SPS, false>), grid, dim3(64 * kW4Waves), 0, stream, a);
     return hipGetLastError();
 }
 
@@ -160,6 +259,25 @@ hipError_t launch_w4(const W4Args& a, bool vec, hipStream_t stream) {
     if (a.group % 128 == 0) return launch_w4<TT, 4>(a, vec, stream);
     if (a.group % 64 == 0) return launch_w4<TT, 2>(a, vec, stream);
     return launch_w4<TT, 1>(a, vec, stream);
+}
+
+hipError_t launch_w4_narrow(const W4Args& a, bool vec, hipStream_t stream) {
+    const uint32_t tiles = kW4Waves / a.split;
+    const dim3 grid((a.row_tiles + tiles - 1u) / tiles);
+    if (vec)
+        hipLaunchKernelGGL(w4_matvec_narrow<true>, grid, dim3(64 * kW4Waves), 0, stream, a);
+    else
+        hipLaunchKernelGGL(w4_matvec_narrow<false>, grid, dim3(64 * kW4Waves), 0, stream, a);
+    return hipGetLastError();
+}
+
+// Waves per row tile: enough for eight waves a CU, no more than there are column tiles.
+uint32_t w4_split(uint32_t row_tiles, uint32_t col_tiles, int cus) {
+    uint32_t split = 1;
+    while (split < kW4Waves && 2u * split <= col_tiles &&
+           (uint64_t)row_tiles * split < 8ull * (uint32_t)cus)
+        split *= 2;
+    return split;
 }
 
 struct W4PackArgs {
@@ -219,7 +337,7 @@ __global__ __launch_bounds__(256) void w4_codes(W4PackArgs a) {
 }
 
 bool w4_sizes_ok(size_t rows, size_t cols, size_t group) {
-    return rows <= 0x7ffffff0u && cols <= (1u << 28) && group > 0 && group % 32 == 0 &&
+    return rows <= 0x7ffffff0u && cols <= (1u << 20) && group > 0 && group % 32 == 0 &&
            group <= 0x7fffffffu;
 }
 
@@ -286,7 +404,18 @@ int attn_w4_matvec(const attn_f16_t* x, attn_f16_t* y, const void* packed,
     a.group = (uint32_t)group_size;
     a.row_tiles = (uint32_t)((out_dim + 15) / 16);
     a.col_tiles = (uint32_t)((in_dim + 127) / 128);
-    const bool vec = aligned16(x) && a.x_stride % 8 == 0 && in_dim % 8 == 0;
+    a.group_mul = group_size >= in_dim
+                      ? 0u
+                      : (uint32_t)(((1ull << 31) + group_size / 32 - 1) / (group_size / 32));
+    int device = 0;
+    const hipError_t e = hipGetDevice(&device);
+    if (e != hipSuccess) return (int)e;
+    a.split = w4_split(a.row_tiles, a.col_tiles, device_cu_count(device));
+    // 16-byte reads of x through one 32-bit range per workgroup
+    const uint64_t x_range = (std::min<uint64_t>(a.tokens, 64) - 1) * a.x_stride + in_dim;
+    const bool vec = aligned16(x) && a.x_stride % 8 == 0 && in_dim % 8 == 0 &&
+                     a.x_stride < (1ull << 31) && x_range * 2 < kDead;
+    if (a.tokens <= 4) return (int)launch_w4_narrow(a, vec, stream);
     if (a.tokens <= 16) return (int)launch_w4<1>(a, vec, stream);
     if (a.tokens <= 32) return (int)launch_w4<2>(a, vec, stream);
     if (a.tokens <= 48) return (int)launch_w4<3>(a, vec, stream);
