@@ -125,7 +125,8 @@ __global__ __launch_bounds__(kTile) void paged_decode_generic(PagedDecodeArgs a)
 constexpr uint32_t kWaves = 4;
 constexpr uint32_t kThreads = 64 * kWaves;
 constexpr uint32_t kUnit = 32;          // keys
-constexpr uint32_t kMinUnits = 8;       // least share of a workgroup: two units a wave
+constexpr uint32_t kMinUnits = 4;       // least share of a workgroup: a unit per wave
+constexpr uint32_t kLead = 4;           // units that the start of a sequence counts for
 constexpr uint32_t kMaxGroups = 512;    // workgroups over all head groups (two per CU)
 constexpr uint32_t kWholeKeys = 384;    // longest table row that takes no split
 constexpr uint32_t kEntries = 1024;     // pool rows staged at once
@@ -157,16 +158,28 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
     return v;
 }
 
-__device__ __forceinline__ uint32_t units_of(const PagedDecodeArgs& a, uint32_t b) {
-    return b < a.num_seqs ? (clamp_len(a.lens[b], a.max_pages, a.page_size) + kUnit - 1u) / kUnit
-                          : 0u;
+__device__ __forceinline__ uint32_t len_of(const PagedDecodeArgs& a, uint32_t b) {
+    return b < a.num_seqs ? clamp_len(a.lens[b], a.max_pages, a.page_size) : 0u;
 }
 
-// A lane's reads of pool rows: BIG through 64-bit addresses; otherwise through a buffer
-// resource over the plane, whose 32-bit offsets take a multiply-add per row, and whose
-// reads of rows that are not live fetch nothing (an offset past the range).  Each byte
-// is read once per call: the non-temporal hint.
-template <bool BIG>
+// Places of a sequence in the line: its units behind a lead, which stands for the time
+// that taking a sequence up costs a workgroup besides its keys (queries, pages, the first
+// loads' latency, the waves' meeting).
+__device__ __forceinline__ uint32_t line_units(uint32_t len) {
+    return len ? (len + kUnit - 1u) / kUnit + kLead : 0u;
+}
+
+// Pools by size: rows below 4 GiB a plane are read through a buffer resource, whose 32-bit
+// offsets take a multiply-add per row and whose reads of rows that are not live fetch
+// nothing (an offset past the range); larger ones through 64-bit addresses.  K and V of a
+// layer that the last-level cache (256 MiB) may keep from one call to the next are read
+// without the non-temporal hint, which else pays off because each byte is read once.  us
+// without / with it: 64 ragged sequences, 353 MB 74.6 / 71.0; 16 of 4 K keys, 134 MB 32.1 /
+// 30.4; one of 32768, 67 MB 18.5 / 20.3; 32 of 64-dim heads, 38 MB 15.0 / 15.5.
+enum { kPoolCached = 0, kPoolStreamed = 1, kPoolHuge = 2 };
+constexpr uint64_t kCachedBytes = 100ull << 20;  // of one K or V plane pair
+
+template <int POOL>
 struct PoolRows {
     const char* base;
     BufRsrc rsrc;
@@ -178,24 +191,25 @@ struct PoolRows {
           lane_bytes(lane) {}
     template <class T>
     __device__ __forceinline__ T get(uint32_t row, uint32_t extra, bool live) const {
-        if constexpr (BIG) {
+        constexpr int AUX = POOL == kPoolCached ? 0 : 2;  // bit 1: non-temporal
+        if constexpr (POOL == kPoolHuge) {
             return __builtin_nontemporal_load(
                 reinterpret_cast<const T*>(base + (uint64_t)row * row_bytes + extra));
         } else {
             const uint32_t at = live ? row * row_bytes + lane_bytes : 0xfffff000u;
             if constexpr (sizeof(T) == 16)
                 return __builtin_bit_cast(
-                    T, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)(at + extra), 0, 2));
+                    T, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)(at + extra), 0, AUX));
             else
                 return __builtin_bit_cast(
-                    T, __builtin_amdgcn_raw_buffer_load_b64(rsrc, (int)(at + extra), 0, 2));
+                    T, __builtin_amdgcn_raw_buffer_load_b64(rsrc, (int)(at + extra), 0, AUX));
         }
     }
 };
 
 // D: head dim (128 or 64).  OCT: the page size is a multiple of 8.  WHOLE: workgroup
-// (head group, sequence) takes the whole sequence.  BIG: a plane of 4 GiB or more.
-template <int D, bool OCT, bool WHOLE, bool BIG>
+// (head group, sequence) takes the whole sequence.
+template <int D, bool OCT, bool WHOLE, int POOL>
 __global__ __launch_bounds__(kThreads, 2) void paged_decode_split(PagedSplitArgs sa) {
     constexpr int kSteps = D / 32;            // MFMAs of a score tile
     constexpr int kTiles = D / 16;            // output tiles, dims {kTiles m + mt}
@@ -218,8 +232,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_split(PagedSplitArgs
     const uint32_t heads = min(16u, a.group - 16u * part);
     const uint32_t row_bytes = a.num_kv_heads * D * 2u;
     const uint64_t plane = (uint64_t)a.num_pages * a.page_size * row_bytes;
-    const PoolRows<BIG> rows_k(a.kp, plane, row_bytes, (g * D + 8u * gq) * 2u);
-    const PoolRows<BIG> rows_v(a.vp, plane, row_bytes, (g * D + (uint32_t)kTiles * n) * 2u);
+    const PoolRows<POOL> rows_k(a.kp, plane, row_bytes, (g * D + 8u * gq) * 2u);
+    const PoolRows<POOL> rows_v(a.vp, plane, row_bytes, (g * D + (uint32_t)kTiles * n) * 2u);
     struct Batch {
         f16x8 k[2][kSteps];
         VRow v[8];
@@ -229,44 +243,51 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_split(PagedSplitArgs
 
     // this workgroup's units [u0, u1) of the line, the sequence that holds u0 and that
     // sequence's first unit
-    uint32_t b, u, u1, base, share = 1;
+    uint32_t b, u, u1, base, len, share = 1;
     if constexpr (WHOLE) {
         b = blockIdx.y;
         u = base = 0;
-        u1 = units_of(a, b);
-        if (u1 == 0) return;
+        len = clamp_len(a.lens[b], a.max_pages, a.page_size);
+        u1 = (len + kUnit - 1u) / kUnit;
     } else {
         uint32_t total = 0;
         for (uint32_t b0 = 0; b0 < a.num_seqs; b0 += 64u)
-            total += (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(units_of(a, b0 + lane)), 63);
-        share = max(kMinUnits, (total + sa.wgs - 1u) / sa.wgs);
-        share = (share + kWaves - 1u) / kWaves * kWaves;  // the same number for each wave
-        if ((uint64_t)w * share >= total) return;
-        u = w * share;
+            total += (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(line_units(len_of(a, b0 + lane))), 63);
+        // the line begins behind the first sequence's lead
+        const uint32_t line = total > kLead ? total - kLead : 0u;
+        share = max(kMinUnits, (line + sa.wgs - 1u) / sa.wgs);
+        if ((uint64_t)w * share >= line) return;
+        u = kLead + w * share;
         u1 = min(total, u + share);
         b = base = 0;
         for (uint32_t b0 = 0;; b0 += 64u) {
-            const uint32_t mine = units_of(a, b0 + lane);
+            const uint32_t mine_len = len_of(a, b0 + lane), mine = line_units(mine_len);
             const uint32_t incl = wave_scan(mine);
             const uint64_t past = __ballot(base + incl > u);
             if (past) {
                 const int at = (int)__builtin_ctzll(past);
                 b = b0 + (uint32_t)at;
                 base += (uint32_t)__builtin_amdgcn_readlane((int)(incl - mine), at);
+                len = (uint32_t)__builtin_amdgcn_readlane((int)mine_len, at);
                 break;
             }
             base += (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
         }
     }
 
+    constexpr uint32_t kSkip = WHOLE ? 0u : kLead;
     while (u < u1) {
-        const uint32_t len = clamp_len(a.lens[b], a.max_pages, a.page_size);
         const uint32_t units = (len + kUnit - 1u) / kUnit;
         if (units == 0) {
             ++b;
+            len = clamp_len(a.lens[b], a.max_pages, a.page_size);
             continue;
         }
-        const uint32_t rel = u - base;                    // first unit of this piece
+        if (u < base + kSkip) {  // the lead of the sequence holds no keys
+            u = base + kSkip;
+            continue;
+        }
+        const uint32_t rel = u - base - kSkip;            // first unit of this piece
         const uint32_t count = min(units - rel, u1 - u);  // its units
         const bool complete = count == units;
 
@@ -372,7 +393,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_split(PagedSplitArgs
             // not fit the registers).
             uint32_t un = wave;
             Batch A, B;
-            if constexpr (BIG) {
+            if constexpr (POOL == kPoolHuge) {
                 for (; un < nu; un += kWaves) {
                     load(un, A);
                     compute(un, A);
@@ -446,29 +467,31 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_split(PagedSplitArgs
         if constexpr (!WHOLE) {
             if (rel == 0 && hg == 0 && tid == 0) {
                 sa.plan[2 * b] = w;
-                sa.plan[2 * b + 1] = (base + units - 1u) / share;
+                sa.plan[2 * b + 1] = (base + units - 1u) / share;  // unit base + lead + units - 1
             }
         }
         __syncthreads();  // the states are read
         u += count;
-        base += units;
+        base += kSkip + units;
         ++b;
+        if (u < u1) len = clamp_len(a.lens[b], a.max_pages, a.page_size);
     }
 }
 
-// Joins the pieces of sequence blockIdx.y for one query head (for a part of its dims):
-// weights of the pieces' maxima, then 4 dims a thread, the pieces shared out over the
-// thread groups.  A sequence in one piece is written already.
+// Joins the pieces of sequence blockIdx.y for one query head (for a part of its dims): the
+// largest maximum, then 4 dims a thread, the pieces shared out over the thread groups.
+// A sequence in one piece is written already.
 template <int D>
 __global__ __launch_bounds__(kThreads) void paged_decode_merge(PagedSplitArgs sa) {
-    __shared__ float s_w[kMaxGroups], s_red[2][kWaves];
-    __shared__ __attribute__((aligned(16))) f32x4 s_x[kThreads];
+    __shared__ float s_max[kWaves];
+    __shared__ __attribute__((aligned(16))) f32x4 s_x[kWaves][D / 4];
+    __shared__ float s_den[kWaves];
     const PagedDecodeArgs& a = sa.d;
-    const uint32_t b = blockIdx.y, tid = threadIdx.x, wave = tid >> 6;
+    const uint32_t b = blockIdx.y, tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
     const uint32_t h = blockIdx.x / sa.dim_parts, dp = blockIdx.x - h * sa.dim_parts;
-    if (units_of(a, b) == 0) return;
-    const uint32_t wf = sa.plan[2 * b], pieces = sa.plan[2 * b + 1] - wf + 1u;
-    if (pieces == 1) return;
+    const uint32_t wf = sa.plan[2 * b], wl = sa.plan[2 * b + 1];  // nothing there without keys
+    const uint32_t pieces = wl - wf + 1u;
+    if (len_of(a, b) == 0 || pieces == 1) return;
     const uint32_t g = h / a.group, in_group = h - g * a.group;
     const uint32_t hg = g * sa.parts + in_group / 16u;
     const uint64_t hg0 = (uint64_t)hg * 2u * sa.wgs;
@@ -476,53 +499,56 @@ __global__ __launch_bounds__(kThreads) void paged_decode_merge(PagedSplitArgs sa
     auto state = [&](uint32_t j) {
         return (hg0 + 2u * (wf + j) + (j == 0 ? 1u : 0u)) * sa.heads + in_group % 16u;
     };
+    // `lanes` threads (4 to 32) hold a state's dims; lane c of a group dims 4 c ..
     const uint32_t lanes = D / 4 / sa.dim_parts, groups = kThreads / lanes;
-    const uint32_t grp = tid / lanes, d = dp * (D / sa.dim_parts) + 4u * (tid - grp * lanes);
-    // the first pieces of each thread, alongside the maxima
+    const uint32_t grp = tid / lanes, c = tid - grp * lanes, d = dp * (D / sa.dim_parts) + 4u * c;
+    // the first pieces of each group, alongside the maxima
     constexpr uint32_t kFirst = 4;
     f32x4 x0[kFirst];
+    float m0[kFirst], l0[kFirst];
 #pragma unroll
     for (uint32_t i = 0; i < kFirst; ++i) {
         const uint32_t j = grp + groups * i;
-        x0[i] = j < pieces ? *reinterpret_cast<const f32x4*>(sa.acc + state(j) * D + d)
-                           : f32x4{0.f, 0.f, 0.f, 0.f};
+        const bool live = j < pieces;
+        const uint64_t st = state(live ? j : 0u);
+        x0[i] = live ? *reinterpret_cast<const f32x4*>(sa.acc + st * D + d)
+                     : f32x4{0.f, 0.f, 0.f, 0.f};
+        m0[i] = live ? sa.m[st] : -INFINITY;
+        l0[i] = live ? sa.l[st] : 0.f;
     }
-    static_assert(kMaxGroups == 2 * kThreads);
-    float m[2], l[2];
-#pragma unroll
-    for (uint32_t i = 0; i < 2; ++i) {
-        const uint32_t j = tid + i * kThreads;
-        m[i] = j < pieces ? sa.m[state(j)] : -INFINITY;
-        l[i] = j < pieces ? sa.l[state(j)] : 0.f;
-    }
-    const float wm = wave_max(fmaxf(m[0], m[1]));
-    if ((tid & 63u) == 0) s_red[0][wave] = wm;
+    float M = -INFINITY;
+    for (uint32_t j = tid; j < pieces; j += kThreads) M = fmaxf(M, sa.m[state(j)]);
+    M = wave_max(M);
+    if (lane == 0) s_max[wave] = M;
     __syncthreads();
-    const float M = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
+    M = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
     float den = 0.f;
 #pragma unroll
-    for (uint32_t i = 0; i < 2; ++i) {
-        const float wt = fast_exp2(m[i] - M);
-        s_w[tid + i * kThreads] = wt;
-        if (tid + i * kThreads < pieces) den += wt * l[i];
-    }
-    den = wave_sum(den);
-    if ((tid & 63u) == 0) s_red[1][wave] = den;
-    __syncthreads();
-    f32x4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
     for (uint32_t i = 0; i < kFirst; ++i) {
-        const uint32_t j = grp + groups * i;
-        if (j < pieces) x += x0[i] * s_w[j];
+        const float wt = fast_exp2(m0[i] - M);  // past the last piece: 0
+        x += x0[i] * wt;
+        den += l0[i] * wt;
     }
 #pragma unroll 4
-    for (uint32_t j = grp + groups * kFirst; j < pieces; j += groups)
-        x += *reinterpret_cast<const f32x4*>(sa.acc + state(j) * D + d) * s_w[j];
-    s_x[tid] = x;
+    for (uint32_t j = grp + groups * kFirst; j < pieces; j += groups) {
+        const uint64_t st = state(j);
+        const float wt = fast_exp2(sa.m[st] - M);
+        x += *reinterpret_cast<const f32x4*>(sa.acc + st * D + d) * wt;
+        den += sa.l[st] * wt;
+    }
+    // the groups of a wave, then the waves
+    for (uint32_t mask = 32; mask >= lanes; mask >>= 1) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] += xor_lane(x[e], (int)mask);
+        den += xor_lane(den, (int)mask);
+    }
+    if (lane < lanes) s_x[wave][lane] = x;
+    if (lane == 0) s_den[wave] = den;
     __syncthreads();
-    if (grp != 0) return;
-    for (uint32_t i = 1; i < groups; ++i) x += s_x[tid + i * lanes];
-    const float inv = 1.0f / ((s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]));
+    if (tid >= lanes) return;
+    x = (s_x[0][tid] + s_x[1][tid]) + (s_x[2][tid] + s_x[3][tid]);
+    const float inv = 1.0f / ((s_den[0] + s_den[1]) + (s_den[2] + s_den[3]));
     const f16x4 o = {(f16)(x[0] * inv), (f16)(x[1] * inv), (f16)(x[2] * inv), (f16)(x[3] * inv)};
     *reinterpret_cast<f16x4*>(a.out + ((uint64_t)b * a.num_heads + h) * D + d) = o;
 }
@@ -552,14 +578,14 @@ PagedPlan paged_plan(size_t num_seqs, size_t num_heads, size_t num_kv_heads, siz
 
 bool paged_split_dim(size_t head_dim) { return head_dim == 128 || head_dim == 64; }
 
-template <int D, bool OCT, bool BIG>
+template <int D, bool OCT, int POOL>
 hipError_t launch_split(const PagedSplitArgs& a, bool whole, hipStream_t stream) {
     if (whole) {
-        hipLaunchKernelGGL((paged_decode_split<D, OCT, true, BIG>),
+        hipLaunchKernelGGL((paged_decode_split<D, OCT, true, POOL>),
                            dim3(a.head_groups, a.d.num_seqs), dim3(kThreads), 0, stream, a);
         return hipGetLastError();
     }
-    hipLaunchKernelGGL((paged_decode_split<D, OCT, false, BIG>), dim3(a.head_groups * a.wgs),
+    hipLaunchKernelGGL((paged_decode_split<D, OCT, false, POOL>), dim3(a.head_groups * a.wgs),
                        dim3(kThreads), 0, stream, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -568,16 +594,20 @@ hipError_t launch_split(const PagedSplitArgs& a, bool whole, hipStream_t stream)
     return hipGetLastError();
 }
 
+template <int D, int POOL>
+hipError_t launch_split(const PagedSplitArgs& a, bool whole, hipStream_t stream) {
+    return a.d.page_size % 8 == 0 ? launch_split<D, true, POOL>(a, whole, stream)
+                                  : launch_split<D, false, POOL>(a, whole, stream);
+}
+
 template <int D>
 hipError_t launch_split(const PagedSplitArgs& a, bool whole, hipStream_t stream) {
+    const uint64_t plane =
+        (uint64_t)a.d.num_pages * a.d.page_size * a.d.num_kv_heads * D * 2;
     // buffer offsets reach 0xffffefff; the ones past it stand for rows that are not read
-    const bool big = (uint64_t)a.d.num_pages * a.d.page_size * a.d.num_kv_heads * D * 2 > 0xffffe000ull;
-    const bool oct = a.d.page_size % 8 == 0;
-    if (big)
-        return oct ? launch_split<D, true, true>(a, whole, stream)
-                   : launch_split<D, false, true>(a, whole, stream);
-    return oct ? launch_split<D, true, false>(a, whole, stream)
-               : launch_split<D, false, false>(a, whole, stream);
+    if (plane > 0xffffe000ull) return launch_split<D, kPoolHuge>(a, whole, stream);
+    if (2 * plane > kCachedBytes) return launch_split<D, kPoolStreamed>(a, whole, stream);
+    return launch_split<D, kPoolCached>(a, whole, stream);
 }
 
 }  // namespace
@@ -624,7 +654,7 @@ int attn_paged_decode(const attn_f16_t* q, const attn_f16_t* k_pages, const attn
     const uint64_t row_units = (max_pages * page_size + kUnit - 1) / kUnit;
     if (paged_split_dim(head_dim) && num_pages > 0 && a.q_stride % 8 == 0 && aligned16(q) &&
         aligned16(k_pages) && aligned16(v_pages) && aligned16(out) &&
-        paged_mul(num_seqs, row_units) <= 0x7fffffffull &&
+        paged_mul(num_seqs, row_units + kLead) <= 0x7fffffffull &&
         get_option(kOptDecodeForceGeneric) == 0) {
         const PagedPlan p = paged_plan(num_seqs, num_heads, num_kv_heads, head_dim);
         PagedSplitArgs sa{};

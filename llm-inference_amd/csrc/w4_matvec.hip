@@ -38,18 +38,29 @@ struct W4Args {
     uint32_t split;        // waves that share a row tile: 1, 2, 4 or 8
 };
 
-// The eight columns of a word as fp16, in order: 1024 + code has the code in its lowest
-// bits, and both it and the difference to 1032 are exact.
+// The eight columns of a word as fp16, in order: code - 8.  With 0x6400 above it a code in
+// the low four bits of a half reads 1024 + code, one in the next four bits 1024 + 16 code:
+// less 1032, or over 16 and less 72, both exact in fp16 (one shift and four masks a word;
+// a shift for every pair took 11 instructions instead of 9).
 __device__ __forceinline__ f16x8 w4_values(uint32_t word) {
-    f16x8 v;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t pair = ((word >> (4 * i)) & 0x000f000fu) | 0x64006400u;
-        const f16x2 x = __builtin_bit_cast(f16x2, pair) - f16x2{(f16)1032.0f, (f16)1032.0f};
-        v[2 * i] = x[0];
-        v[2 * i + 1] = x[1];
-    }
-    return v;
+    const uint32_t up = word >> 8;
+    const f16x2 c0 = __builtin_bit_cast(f16x2, (word & 0x000f000fu) | 0x64006400u);
+    const f16x2 c1 = __builtin_bit_cast(f16x2, (word & 0x00f000f0u) | 0x64006400u);
+    const f16x2 c2 = __builtin_bit_cast(f16x2, (up & 0x000f000fu) | 0x64006400u);
+    const f16x2 c3 = __builtin_bit_cast(f16x2, (up & 0x00f000f0u) | 0x64006400u);
+    const f16x2 low = {(f16)-1032.0f, (f16)-1032.0f}, high = {(f16)-72.0f, (f16)-72.0f};
+    const f16x2 part = {(f16)0.0625f, (f16)0.0625f};
+    const f16x2 v0 = c0 + low, v2 = c2 + low;
+    const f16x2 v1 = __builtin_elementwise_fma(c1, part, high);
+    const f16x2 v3 = __builtin_elementwise_fma(c3, part, high);
+    return f16x8{v0[0], v0[1], v1[0], v1[1], v2[0], v2[1], v3[0], v3[1]};
+}
+
+// 16 bytes of codes per lane.  Without the non-temporal hint: 64 tokens, 12000 x 12000
+// 50 us against 60 with it, one token, 128256 x 2048 (HBM-cold) level.
+__device__ __forceinline__ u32x4 w4_load(BufRsrc rows, uint32_t byte_off) {
+    return __builtin_bit_cast(u32x4,
+                              __builtin_amdgcn_raw_buffer_load_b128(rows, (int)byte_off, 0, 0));
 }
 
 constexpr uint32_t kW4Waves = 8;
@@ -64,14 +75,14 @@ __device__ __forceinline__ uint32_t w4_group(const W4Args& a, uint32_t k) {
 
 // Sums of the waves that share a row tile: `part` waves (a power of two) of the workgroup's
 // eight, wave-contiguous.  s_part is [wave][tokens][17].
-template <int TOKENS>
-__device__ __forceinline__ void w4_store(const W4Args& a, const float (*s_part)[TOKENS][17],
+template <int TOKENS, int R>
+__device__ __forceinline__ void w4_store(const W4Args& a, const float (*s_part)[TOKENS][16 * R + 1],
                                          uint32_t t0, uint32_t live) {
     const uint32_t tiles = kW4Waves / a.split, first = blockIdx.x * tiles;
-    const uint32_t per_tile = live * 16u;
+    const uint32_t per_tile = live * 16u * R;
     for (uint32_t i = threadIdx.x; i < tiles * per_tile; i += 64u * kW4Waves) {
         const uint32_t tile = i / per_tile, j = i - tile * per_tile;
-        const uint32_t t = j >> 4, r = j & 15u, row = (first + tile) * 16u + r;
+        const uint32_t t = j / (16u * R), r = j % (16u * R), row = (first + tile) * 16u * R + r;
         if (row >= a.rows) continue;
         float sum = 0.f;
         for (uint32_t x = 0; x < a.split; ++x) sum += s_part[tile * a.split + x][t][r];
@@ -110,8 +121,7 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matvec_narrow(W4Args a) {
             f16x4 scale;
         } st[kDepth];
         auto load = [&](uint32_t c, Stage& z) {
-            z.w = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                                                rw, (int)(c * 1024u + 16u * lane), 0, 2));
+            z.w = w4_load(rw, c * 1024u + 16u * lane);
             const uint32_t k = 128u * c + 32u * step + 8u * gq;
             if constexpr (VEC) {
                 z.x = buf_ld16(rx, k < a.cols ? x_at + 2u * k : kDead);
@@ -149,64 +159,130 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matvec_narrow(W4Args a) {
         if (step == 0) s_part[wave][n >> 2][4u * gq + r] = v;
     }
     __syncthreads();
-    w4_store<4>(a, s_part, 0, a.tokens);
+    w4_store<4, 1>(a, s_part, 0, a.tokens);
 }
 
-// Any number of tokens, TT tiles of 16 at a time.  SPS: steps of 32 columns that share a
-// scale at least (4: the group is a multiple of 128; 2: of 64; 1).  The products of a
-// scale's columns are summed by the MFMAs from zero, then scaled and added in fp32, so no
-// product is rounded.
-template <int TT, int SPS, bool VEC>
+// the scales that lane step % 4 of each four lanes loaded, in all four
+template <int S>
+__device__ __forceinline__ f16x4 w4_step_scale(u32x2 mine) {
+    u32x2 v;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)  // quad_perm [S, S, S, S]
+        v[i] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)mine[i], S * 0x55, 0xF, 0xF, false);
+    return __builtin_bit_cast(f16x4, v);
+}
+
+// Any number of tokens: R row tiles x TT tiles of 16 tokens a wave.  SPS: steps of 32
+// columns that share a scale at least (4: the group is a multiple of 128; 2: of 64; 1).
+// The products of a scale's columns are summed by the MFMAs from zero, then scaled and
+// added in fp32, so no product is rounded.
+template <int R, int TT, int SPS, bool VEC>
 __global__ __launch_bounds__(64 * kW4Waves) void w4_matvec(W4Args a) {
-    constexpr int kDepth = TT == 1 ? 4 : 2;  // column tiles in flight
-    __shared__ float s_part[kW4Waves][16 * TT][17];
+    constexpr int kDepth = VEC ? 2 : 1;  // column tiles in flight
+    // a wave's x tile (16 tokens x 128 columns each), then the waves' sums
+    union Shared {
+        f16x8 x[kW4Waves][TT][256];
+        float part[kW4Waves][16 * TT][16 * R + 1];
+    };
+    __shared__ __attribute__((aligned(16))) Shared s_mem;
     const uint32_t lane = threadIdx.x & 63u;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t n = lane & 15u, gq = lane >> 4;
-    const uint32_t rt = (blockIdx.x * kW4Waves + wave) / a.split;
+    const uint32_t rt = (blockIdx.x * kW4Waves + wave) / a.split * R;
     const uint32_t first = wave & (a.split - 1u);
     const uint32_t t0 = blockIdx.y * 16u * TT;
     const uint32_t live = min(a.tokens - t0, 16u * (uint32_t)TT);
-    f32x4 acc[TT];
+    f32x4 acc[R][TT];
 #pragma unroll
-    for (int tt = 0; tt < TT; ++tt) acc[tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int q = 0; q < R; ++q)
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) acc[q][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (rt < a.row_tiles && a.col_tiles > 0) {
-        const BufRsrc rw =
-            make_rsrc(a.w + (uint64_t)rt * a.col_tiles * 256u, a.col_tiles * 1024u);
+        // row tiles past the last one read nothing
+        const uint32_t tile_bytes = a.col_tiles * 1024u;
+        BufRsrc rw[R];
+        const f16* sc[R];
+        const uint64_t sc_stride = (uint64_t)a.row_tiles * 16u;
+#pragma unroll
+        for (int q = 0; q < R; ++q) {
+            const uint32_t r = min(rt + q, a.row_tiles - 1u);
+            rw[q] = make_rsrc(a.w + (uint64_t)r * a.col_tiles * 256u, tile_bytes);
+            sc[q] = a.scales + r * 16u + 4u * gq;
+        }
         const f16* const xb = a.x + (uint64_t)t0 * a.x_stride;
         const BufRsrc rx = make_rsrc(xb, (uint32_t)(((live - 1u) * a.x_stride + a.cols) * 2u));
-        uint64_t x_at[TT];  // elements
+        // x is read in whole lines, four rows of 256 bytes an instruction (16 rows of 64
+        // bytes, as the MFMA operand wants it, took the load pipe twice as long), and turned
+        // in LDS: row r's 16-byte chunk i lies at chunk i ^ r, so that the 16 rows of an
+        // operand read cover all banks.
+        uint64_t x_at[TT][4];  // elements; tokens past the last repeat it: nothing of theirs is stored
 #pragma unroll
-        for (int tt = 0; tt < TT; ++tt)  // lanes past the last token repeat it; nothing of theirs is stored
-            x_at[tt] = min(16u * tt + n, live - 1u) * a.x_stride;
-        const f16* const sc = a.scales + rt * 16u + 4u * gq;
-        const uint64_t sc_stride = (uint64_t)a.row_tiles * 16u;
+        for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j)
+                x_at[tt][j] = min(16u * tt + 4u * j + gq, live - 1u) * a.x_stride + 8u * n;
         struct Stage {
-            u32x4 w;
-            f16x8 x[4][TT];
-            f16x4 scale[4 / SPS];
+            u32x4 w[R];
+            f16x8 x[TT][4];
+            u32x2 scale[R];  // of step n % 4, rows 4 gq ..
         } st[kDepth];
         auto load = [&](uint32_t c, Stage& z) {
-            z.w = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                                                rw, (int)(c * 1024u + 16u * lane), 0, 2));
+            const uint64_t at = w4_group(a, min(128u * c + 32u * (n & 3u), a.cols - 1u)) * sc_stride;
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const uint32_t k = 128u * c + 32u * s + 8u * gq;
-                if (s % SPS == 0)
-                    z.scale[s / SPS] = *reinterpret_cast<const f16x4*>(
-                        sc + w4_group(a, min(128u * c + 32u * s, a.cols - 1u)) * sc_stride);
+            for (int q = 0; q < R; ++q) {
+                z.w[q] = w4_load(rw[q], c * 1024u + 16u * lane);
+                z.scale[q] = *reinterpret_cast<const u32x2*>(sc[q] + at);
+            }
+            const uint32_t k = 128u * c + 8u * n;
 #pragma unroll
-                for (int tt = 0; tt < TT; ++tt) {
+            for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) {
                     if constexpr (VEC) {
-                        z.x[s][tt] =
-                            buf_ld16(rx, k < a.cols ? 2u * ((uint32_t)x_at[tt] + k) : kDead);
+                        z.x[tt][j] = buf_ld16(
+                            rx, k < a.cols ? 2u * ((uint32_t)x_at[tt][j] + 128u * c) : kDead);
                     } else {
 #pragma unroll
                         for (uint32_t e = 0; e < 8; ++e)
-                            z.x[s][tt][e] = k + e < a.cols ? xb[x_at[tt] + k + e] : (f16)0.f;
+                            z.x[tt][j][e] =
+                                k + e < a.cols ? xb[x_at[tt][j] + 128u * c + e] : (f16)0.f;
                     }
                 }
-            }
+        };
+        auto compute = [&](const Stage& z) {
+#pragma unroll
+            for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) {
+                    const uint32_t r = 4u * j + gq;
+                    s_mem.x[wave][tt][16u * r + (n ^ r)] = z.x[tt][j];
+                }
+            f32x4 part[R][TT];
+            auto step = [&]<int s>() {
+                f16x8 xv[TT];
+#pragma unroll
+                for (int tt = 0; tt < TT; ++tt)
+                    xv[tt] = s_mem.x[wave][tt][16u * n + ((4u * s + gq) ^ n)];
+#pragma unroll
+                for (int q = 0; q < R; ++q) {
+                    const f16x8 wv = w4_values(z.w[q][s]);
+                    const f16x4 scale = w4_step_scale<s>(z.scale[q]);
+#pragma unroll
+                    for (int tt = 0; tt < TT; ++tt) {
+                        if (s % SPS == 0) part[q][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+                        part[q][tt] = mfma16(wv, xv[tt], part[q][tt]);
+                        if (s % SPS == SPS - 1)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                acc[q][tt][r] =
+                                    __builtin_fmaf((float)scale[r], part[q][tt][r], acc[q][tt][r]);
+                    }
+                }
+            };
+            step.template operator()<0>();
+            step.template operator()<1>();
+            step.template operator()<2>();
+            step.template operator()<3>();
         };
 #pragma unroll
         for (int i = 0; i < kDepth; ++i) load(first + i * a.split, st[i]);
@@ -214,51 +290,41 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matvec(W4Args a) {
 #pragma unroll
             for (int i = 0; i < kDepth; ++i) {
                 __builtin_amdgcn_sched_barrier(0);
-                if (c + i * a.split < a.col_tiles) {
-                    f32x4 part[TT];
-#pragma unroll
-                    for (int s = 0; s < 4; ++s) {
-                        const f16x8 wv = w4_values(st[i].w[s]);
-#pragma unroll
-                        for (int tt = 0; tt < TT; ++tt) {
-                            if (s % SPS == 0) part[tt] = f32x4{0.f, 0.f, 0.f, 0.f};
-                            part[tt] = mfma16(wv, st[i].x[s][tt], part[tt]);
-                            if (s % SPS == SPS - 1)
-#pragma unroll
-                                for (int r = 0; r < 4; ++r)
-                                    acc[tt][r] = __builtin_fmaf((float)st[i].scale[s / SPS][r],
-                                                                part[tt][r], acc[tt][r]);
-                        }
-                    }
-                }
+                if (c + i * a.split < a.col_tiles) compute(st[i]);
                 load(c + (i + kDepth) * a.split, st[i]);
             }
         }
     }
+    __syncthreads();  // every wave has read its x tiles
 #pragma unroll
-    for (int tt = 0; tt < TT; ++tt)
+    for (int q = 0; q < R; ++q)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s_part[wave][16 * tt + n][4u * gq + r] = acc[tt][r];
+        for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                s_mem.part[wave][16 * tt + n][16 * q + 4u * gq + r] = acc[q][tt][r];
     __syncthreads();
-    w4_store<16 * TT>(a, s_part, t0, live);
+    w4_store<16 * TT, R>(a, s_mem.part, t0, live);
 }
 
-template <int TT, int SPS>
+template <int R, int TT, int SPS>
 hipError_t launch_w4(const W4Args& a, bool vec, hipStream_t stream) {
-    const uint32_t tiles = kW4Waves / a.split;
+    const uint32_t tiles = kW4Waves / a.split * R;
     const dim3 grid((a.row_tiles + tiles - 1u) / tiles, (a.tokens + 16u * TT - 1u) / (16u * TT));
     if (vec)
-        hipLaunchKernelGGL((w4_matvec<TT, SPS, true>), grid, dim3(64 * kW4Waves), 0, stream, a);
+        hipLaunchKernelGGL((w4_matvec<R, TT, SPS, true>), grid, dim3(64 * kW4Waves), 0, stream, a);
+    else if constexpr (TT == 1)  // two token tiles of element-wise loads spill
+        hipLaunchKernelGGL((w4_matvec<R, TT, SPS, false>), grid, dim3(64 * kW4Waves), 0, stream, a);
     else
-        hipLaunchKernelGGL((w4_matvec<TT, SPS, false>), grid, dim3(64 * kW4Waves), 0, stream, a);
+        return hipErrorInvalidValue;
     return hipGetLastError();
 }
 
-template <int TT>
+template <int R, int TT>
 hipError_t launch_w4(const W4Args& a, bool vec, hipStream_t stream) {
-    if (a.group % 128 == 0) return launch_w4<TT, 4>(a, vec, stream);
-    if (a.group % 64 == 0) return launch_w4<TT, 2>(a, vec, stream);
-    return launch_w4<TT, 1>(a, vec, stream);
+    if (a.group % 128 == 0) return launch_w4<R, TT, 4>(a, vec, stream);
+    if (a.group % 64 == 0) return launch_w4<R, TT, 2>(a, vec, stream);
+    return launch_w4<R, TT, 1>(a, vec, stream);
 }
 
 hipError_t launch_w4_narrow(const W4Args& a, bool vec, hipStream_t stream) {
@@ -271,11 +337,13 @@ hipError_t launch_w4_narrow(const W4Args& a, bool vec, hipStream_t stream) {
     return hipGetLastError();
 }
 
-// Waves per row tile: enough for eight waves a CU, no more than there are column tiles.
-uint32_t w4_split(uint32_t row_tiles, uint32_t col_tiles, int cus) {
+// Waves per row tile, no more than there are column tiles.  Narrow: enough for eight waves
+// a CU.  Otherwise as many as there are (33 tokens, 2048 x 11008: 14 us with eight, 23 with
+// four; 64 tokens, 12000 x 12000: 59-61 with either).
+uint32_t w4_split(uint32_t row_tiles, uint32_t col_tiles, bool narrow, int cus) {
     uint32_t split = 1;
     while (split < kW4Waves && 2u * split <= col_tiles &&
-           (uint64_t)row_tiles * split < 8ull * (uint32_t)cus)
+           (!narrow || (uint64_t)row_tiles * split < 8ull * (uint32_t)cus))
         split *= 2;
     return split;
 }
@@ -410,16 +478,27 @@ int attn_w4_matvec(const attn_f16_t* x, attn_f16_t* y, const void* packed,
     int device = 0;
     const hipError_t e = hipGetDevice(&device);
     if (e != hipSuccess) return (int)e;
-    a.split = w4_split(a.row_tiles, a.col_tiles, device_cu_count(device));
+    a.split = w4_split(a.row_tiles, a.col_tiles, a.tokens <= 4, device_cu_count(device));
     // 16-byte reads of x through one 32-bit range per workgroup
     const uint64_t x_range = (std::min<uint64_t>(a.tokens, 64) - 1) * a.x_stride + in_dim;
     const bool vec = aligned16(x) && a.x_stride % 8 == 0 && in_dim % 8 == 0 &&
                      a.x_stride < (1ull << 31) && x_range * 2 < kDead;
     if (a.tokens <= 4) return (int)launch_w4_narrow(a, vec, stream);
-    if (a.tokens <= 16) return (int)launch_w4<1>(a, vec, stream);
-    if (a.tokens <= 32) return (int)launch_w4<2>(a, vec, stream);
-    if (a.tokens <= 48) return (int)launch_w4<3>(a, vec, stream);
-    return (int)launch_w4<4>(a, vec, stream);
+    // Row and token tiles of a wave, by what gives every CU a workgroup (us; tokens x rows x
+    // columns):       1 row tile, 1 token tile   2, 1    4, 2
+    //  16 x 2048 x 2048                     3.9   4.5     8.0
+    //  40 x 500 x 8000                      7.2   9.7    19.3
+    //  33 x 2048 x 11008                   14.4  12.5    23.8
+    //  16 x 12000 x 12000                  25.3  23.0    26.2
+    //  33 x 11008 x 2048                   16.1  13.3    16.3
+    //  64 x 12000 x 12000                  83.4  58.9    50.4
+    const uint64_t cus = (uint32_t)device_cu_count(device);
+    const uint64_t token_tiles = (a.tokens + 15u) / 16u;
+    const uint64_t pairs = (a.tokens + 31u) / 32u;  // of token tiles
+    if (vec && a.tokens > 32 && 32u * pairs - a.tokens < 16u && (a.row_tiles + 3u) / 4u * pairs >= cus)
+        return (int)launch_w4<4, 2>(a, vec, stream);
+    if (a.row_tiles * token_tiles >= cus) return (int)launch_w4<2, 1>(a, vec, stream);
+    return (int)launch_w4<1, 1>(a, vec, stream);
 }
 
 }  // extern "C"

@@ -145,15 +145,20 @@ def exported_symbols():
 
 
 def _ptr(x) -> Optional[int]:
-    if x is None:
-        return None
-    if isinstance(x, int):
+    if x is None or isinstance(x, int):
         return x
     return x.data_ptr()
 
 
+# The current stream's handle without the Stream object around it (a call of a wrapper
+# costs the host a few microseconds, as much as a short kernel takes).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream(stream) -> Optional[int]:
     if stream is None:
+        if _raw_stream is not None and torch.cuda.is_initialized():
+            return _raw_stream(torch.cuda.current_device())
         return torch.cuda.current_stream().cuda_stream
     if isinstance(stream, int):
         return stream

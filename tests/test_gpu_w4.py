@@ -114,6 +114,16 @@ def test_the_layers_of_a_model(attn, gpu):
             product(attn, gpu, T, N, K, group, T, residual="apart")
 
 
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("T,N,K", [(64, 8200, 160), (50, 8208, 200), (100, 6000, 96),
+                                   (64, 8200, 164),   # columns that take element loads
+                                   (16, 4100, 300), (40, 1500, 256)])
+def test_many_rows(attn, gpu, T, N, K, group):
+    """The tiles of more rows and tokens a wave, rows and tokens that end inside them."""
+    print(f"[case] T={T} N={N} K={K} group={group}", flush=True)
+    product(attn, gpu, T, N, K, group, T, residual="apart")
+
+
 def test_infinity_in_one_token_stays_there(attn, gpu):
     N, K = 40, 200
     codes, scales = weights(N, K, 32, 1)
