@@ -16,7 +16,7 @@
 // sequence, some whole ones and the start of another: whole ones are written to the
 // output at once, pieces to the workspace as fp32 states (running maximum, sum,
 // unnormalised output), and a second kernel joins a sequence's pieces.  Where no table
-// row can hold more than kWholeKeys keys, a workgroup per sequence and KV head and no
+// row can hold more than a few hundred keys, a workgroup per sequence and KV head and no
 // second kernel.
 //
 // A unit.  Four waves take units in turn, each with two in flight.  Scores are S^T = K
@@ -128,7 +128,9 @@ constexpr uint32_t kUnit = 32;          // keys
 constexpr uint32_t kMinUnits = 4;       // least share of a workgroup: a unit per wave
 constexpr uint32_t kLead = 4;           // units that the start of a sequence counts for
 constexpr uint32_t kMaxGroups = 512;    // workgroups over all head groups (two per CU)
-constexpr uint32_t kWholeKeys = 384;    // longest table row that takes no split
+// longest table rows that take no split: any batch, and batches that give half the CUs a
+// workgroup (see attn_paged_decode)
+constexpr uint32_t kWholeKeys = 512, kWholeKeysBatch = 1024;
 constexpr uint32_t kEntries = 1024;     // pool rows staged at once
 constexpr float kNoMax = -1.0e30f;      // finite: masked scores (-inf) get weight 0
 constexpr float kWeightBits = 15.0f;
@@ -670,7 +672,18 @@ int attn_paged_decode(const attn_f16_t* q, const attn_f16_t* k_pages, const attn
         sa.wgs = p.wgs;
         // few sequences: more workgroups of fewer dims each join a long one's pieces
         sa.dim_parts = num_seqs * num_heads < 128 ? 4u : 1u;
-        const bool whole = max_pages * page_size <= kWholeKeys;
+        // One kernel, a workgroup per sequence and KV head, against two (us, 16/4 heads of
+        // 128, rows of up to as many keys).  500 keys: 7.8 / 8.4 for one sequence, 10.7 / 15.9
+        // for 64; 1000 keys: 12.0 / 8.4, 13.0 / 11.2 for 16, 13.7 / 14.7 for 32, 17.2 / 21.2 for
+        // 64; 2000 keys: 40.7 / 37.9 for 64.
+        const uint64_t keys = max_pages * page_size;
+        int device = 0;
+        const hipError_t e = hipGetDevice(&device);
+        if (e != hipSuccess) return (int)e;
+        const bool whole =
+            keys <= kWholeKeys ||
+            (keys <= kWholeKeysBatch &&
+             2 * num_seqs * p.head_groups >= (uint64_t)device_cu_count(device));
         return (int)(head_dim == 128 ? launch_split<128>(sa, whole, stream)
                                      : launch_split<64>(sa, whole, stream));
     }

@@ -70,14 +70,28 @@ class Case:
                 assert (err <= bound).all(), (b, n, g, err.max(), (err / bound).max())
 
 
+# how a call is split: table rows of a few hundred keys take one kernel, wide ones two; the
+# generic kernel is the one of other head dims and unaligned tensors
+@pytest.fixture(params=["one kernel", "two kernels", "generic"])
+def form(request, attn):
+    attn.set_option("decode_force_generic", int(request.param == "generic"))
+    yield request.param
+    attn.set_option("decode_force_generic", 0)
+
+
+def columns_of(form, page, high):
+    return -(-5000 // page) if form == "two kernels" else -(-high // page) + 1
+
+
 # lengths around 8, 16, 32, 64 and the page's end
 LENS = [1, 0, 7, 8, 9, 31, 32, 33, 63, 64, 65, 100, 127, 129, 254, 300]
 
 
 @pytest.mark.parametrize("page", [1, 3, 8, 16, 24, 32, 64, 100, 128])
 @pytest.mark.parametrize("Hq,Hkv,D", [(16, 4, 128), (16, 4, 64)])
-def test_pages_and_lengths(attn, gpu, page, Hq, Hkv, D):
-    c = Case(attn, gpu, LENS, page, Hq, Hkv, D, seed=page)
+def test_pages_and_lengths(attn, gpu, form, page, Hq, Hkv, D):
+    c = Case(attn, gpu, LENS, page, Hq, Hkv, D, seed=page,
+             columns=columns_of(form, page, max(LENS)))
     c.call()
     c.check(c.got())
 
@@ -103,11 +117,12 @@ def test_long_sequences(attn, gpu, Hq, Hkv, D, page, lens):
     c.check(c.got())
 
 
-@pytest.mark.parametrize("B,high", [(200, 60), (70, 900), (1100, 9)])
-def test_many_sequences(attn, gpu, B, high):
+@pytest.mark.parametrize("columns", [None, 100])
+@pytest.mark.parametrize("B,high", [(200, 60), (70, 900), (1100, 9), (64, 40), (65, 40)])
+def test_many_sequences(attn, gpu, B, high, columns):
     rng = np.random.default_rng(B)
     lens = rng.integers(0, high + 1, B).tolist()
-    c = Case(attn, gpu, lens, 16, 8, 2, 128, seed=B)
+    c = Case(attn, gpu, lens, 16, 8, 2, 128, seed=B, columns=columns)
     c.call()
     c.check(c.got())
 
@@ -143,10 +158,11 @@ def test_many_small_weights_keep_their_sum(attn, gpu, D):
     c.check(c.got())
 
 
-def test_infinities_and_nan_stay_where_they_are(attn, gpu):
+def test_infinities_and_nan_stay_where_they_are(attn, gpu, form):
     """A NaN in V reaches its dim of its KV head's queries of its sequence, a NaN in K
     that head's queries, an infinite V its dim; other sequences are as they would be."""
-    c = Case(attn, gpu, [200, 200, 200, 200], 16, 8, 2, 128, seed=8)
+    c = Case(attn, gpu, [200, 200, 200, 200], 16, 8, 2, 128, seed=8,
+             columns=columns_of(form, 16, 200))
     c.v[c.lay.rows(0)[150], 1, 7] = np.nan
     c.k[c.lay.rows(1)[3], 0, 9] = np.nan
     c.v[c.lay.rows(2)[199], 0, 100] = np.inf
@@ -163,10 +179,10 @@ def test_infinities_and_nan_stay_where_they_are(attn, gpu):
 
 @pytest.mark.parametrize("bad", [-1, 2**30, -2**31])
 @pytest.mark.parametrize("at", [0, 5, 18])
-def test_page_out_of_range(attn, gpu, bad, at):
+def test_page_out_of_range(attn, gpu, form, bad, at):
     """Its sequence is NaN, the others are not touched by it; entries past a sequence's
     end are never used (the layout fills them with numbers out of range)."""
-    c = Case(attn, gpu, [300, 300, 33], 16, 16, 4, 128, seed=9)
+    c = Case(attn, gpu, [300, 300, 33], 16, 16, 4, 128, seed=9, columns=columns_of(form, 16, 300))
     c.table[1, at] = bad
     c.call()
     got = c.got()
@@ -174,12 +190,13 @@ def test_page_out_of_range(attn, gpu, bad, at):
     c.check(got, skip=(1,))
 
 
-def test_lengths_past_the_table_are_cut(attn, gpu):
-    c = Case(attn, gpu, [64, 32], 16, 16, 4, 128, seed=10, columns=4)
+@pytest.mark.parametrize("keys", [64, 1600])
+def test_lengths_past_the_table_are_cut(attn, gpu, keys):
+    c = Case(attn, gpu, [keys, 32], 16, 16, 4, 128, seed=10, columns=keys // 16)
     c.lens[0] = 2**31 - 1
     c.lens[1] = -5
     c.call()
-    c.check(c.got(), lens=[64, 0])
+    c.check(c.got(), lens=[keys, 0])
 
 
 def test_captured_call_with_changing_lengths(attn, gpu):
@@ -211,6 +228,12 @@ def test_captured_call_with_changing_lengths(attn, gpu):
         hipgraph.destroy(*g)
 
 
+def test_batch_without_keys(attn, gpu, form):
+    c = Case(attn, gpu, [0] * 70, 16, 8, 2, 128, seed=15, columns=columns_of(form, 16, 400))
+    c.call()
+    assert (c.got() == OUT).all()
+
+
 def test_same_bits_every_time(attn, gpu):
     c = Case(attn, gpu, [5000, 123, 1], 16, 16, 4, 128, seed=13)
     c.call()
@@ -222,7 +245,8 @@ def test_same_bits_every_time(attn, gpu):
         assert np.array_equal(c.got(), first)
 
 
-def test_pool_past_four_gigabytes(attn, gpu):
+@pytest.mark.parametrize("columns", [8, 100])
+def test_pool_past_four_gigabytes(attn, gpu, columns):
     """Pages whose byte offset passes 32 bits: 2^21 rows of 4 KiB in each of K and V,
     sequences on the pool's last pages and its first."""
     Hq, Hkv, D, page, pages = 16, 16, 128, 16, 2**17
@@ -232,7 +256,7 @@ def test_pool_past_four_gigabytes(attn, gpu):
     k = torch.empty(rows, Hkv, D, dtype=torch.float16, device=gpu)
     v = torch.empty_like(k)
     lens = [100, 33]
-    table = np.full((2, 8), -1, dtype=np.int32)
+    table = np.full((2, columns), -1, dtype=np.int32)
     table[0, :7] = [pages - 1, 0, pages - 2, 2**16, 3, pages - 9, 2**16 - 1]
     table[1, :3] = [2**16 + 1, 5, pages - 5]
     rng = np.random.default_rng(14)
@@ -248,7 +272,7 @@ def test_pool_past_four_gigabytes(attn, gpu):
     out = torch.empty(2, Hq, D, dtype=torch.float16, device=gpu)
     ws = attn.paged_decode_workspace(2, Hq, Hkv, D, gpu)
     attn.paged_decode(torch.from_numpy(q).to(gpu), k, v, out, torch.from_numpy(table).to(gpu),
-                      torch.tensor(lens, dtype=torch.int32, device=gpu), 2, 8, pages, page, Hq,
+                      torch.tensor(lens, dtype=torch.int32, device=gpu), 2, columns, pages, page, Hq,
                       Hkv, D, ws)
     torch.cuda.synchronize()
     got = out.cpu().numpy().astype(np.float64)
@@ -256,3 +280,13 @@ def test_pool_past_four_gigabytes(attn, gpu):
         for g in range(Hkv):
             exp, bound = ref.decode(q[b, g:g + 1], held[b][0][:, g], held[b][1][:, g], D**-0.5)
             assert (np.abs(got[b, g] - exp[0]) <= bound[0]).all()
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,page", [(16, 4, 128, 16), (16, 4, 64, 7)])
+@pytest.mark.parametrize("columns", [40, 1000])
+def test_pool_that_no_cache_keeps(attn, gpu, Hq, Hkv, D, page, columns):
+    """K and V of more than 100 MiB, which are read with another hint."""
+    spare = 110 * 2**20 // (4 * Hkv * D * page)
+    c = Case(attn, gpu, [260, 3, 0, 100], page, Hq, Hkv, D, seed=16, columns=columns, spare=spare)
+    c.call()
+    c.check(c.got())
