@@ -40,14 +40,22 @@ struct W4Args {
 
 // The eight columns of a word as fp16, in order: code - 8.  With 0x6400 above it a code in
 // the low four bits of a half reads 1024 + code, one in the next four bits 1024 + 16 code:
-// less 1032, or over 16 and less 72, both exact in fp16 (one shift and four masks a word;
-// a shift for every pair took 11 instructions instead of 9).
-__device__ __forceinline__ f16x8 w4_values(uint32_t word) {
+// less 1032, or over 16 and less 72, both exact in fp16.  The constants live in registers
+// (hidden from the compiler), so that mask and or are one v_and_or_b32, which takes no
+// literals: 9 instructions a word, 13 otherwise (33 tokens, 2048 x 11008,
+// groups of 32: 14.4 us against 15.1).
+struct W4Consts {
+    uint32_t low, high, one;
+    __device__ W4Consts() : low(0x000f000fu), high(0x00f000f0u), one(0x64006400u) {
+        asm("" : "+s"(low), "+s"(high), "+v"(one));
+    }
+};
+__device__ __forceinline__ f16x8 w4_values(uint32_t word, const W4Consts& k) {
     const uint32_t up = word >> 8;
-    const f16x2 c0 = __builtin_bit_cast(f16x2, (word & 0x000f000fu) | 0x64006400u);
-    const f16x2 c1 = __builtin_bit_cast(f16x2, (word & 0x00f000f0u) | 0x64006400u);
-    const f16x2 c2 = __builtin_bit_cast(f16x2, (up & 0x000f000fu) | 0x64006400u);
-    const f16x2 c3 = __builtin_bit_cast(f16x2, (up & 0x00f000f0u) | 0x64006400u);
+    const f16x2 c0 = __builtin_bit_cast(f16x2, (word & k.low) | k.one);
+    const f16x2 c1 = __builtin_bit_cast(f16x2, (word & k.high) | k.one);
+    const f16x2 c2 = __builtin_bit_cast(f16x2, (up & k.low) | k.one);
+    const f16x2 c3 = __builtin_bit_cast(f16x2, (up & k.high) | k.one);
     const f16x2 low = {(f16)-1032.0f, (f16)-1032.0f}, high = {(f16)-72.0f, (f16)-72.0f};
     const f16x2 part = {(f16)0.0625f, (f16)0.0625f};
     const f16x2 v0 = c0 + low, v2 = c2 + low;
@@ -103,6 +111,7 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matvec_narrow(W4Args a) {
     const uint32_t lane = threadIdx.x & 63u;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t n = lane & 15u, gq = lane >> 4, step = n & 3u;
+    const W4Consts consts;
     const uint32_t rt = (blockIdx.x * kW4Waves + wave) / a.split;
     const uint32_t first = wave & (a.split - 1u);
     const uint32_t token = min(n >> 2, a.tokens - 1u);
@@ -142,7 +151,7 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matvec_narrow(W4Args a) {
                     f32x4 part = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (uint32_t s = 0; s < 4; ++s)
-                        part = mfma16(w4_values(st[i].w[s]), step == s ? st[i].x : f16x8{}, part);
+                        part = mfma16(w4_values(st[i].w[s], consts), step == s ? st[i].x : f16x8{}, part);
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
                         acc[r] = __builtin_fmaf((float)st[i].scale[r], part[r], acc[r]);
@@ -191,6 +200,7 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matvec(W4Args a) {
     const uint32_t rt = (blockIdx.x * kW4Waves + wave) / a.split * R;
     const uint32_t first = wave & (a.split - 1u);
     const uint32_t t0 = blockIdx.y * 16u * TT;
+    const W4Consts consts;
     const uint32_t live = min(a.tokens - t0, 16u * (uint32_t)TT);
     f32x4 acc[R][TT];
 #pragma unroll
@@ -265,7 +275,7 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matvec(W4Args a) {
                     xv[tt] = s_mem.x[wave][tt][16u * n + ((4u * s + gq) ^ n)];
 #pragma unroll
                 for (int q = 0; q < R; ++q) {
-                    const f16x8 wv = w4_values(z.w[q][s]);
+                    const f16x8 wv = w4_values(z.w[q][s], consts);
                     const f16x4 scale = w4_step_scale<s>(z.scale[q]);
 #pragma unroll
                     for (int tt = 0; tt < TT; ++tt) {
