@@ -117,7 +117,8 @@ int attn_update_merge_node(hipGraphExec_t graph_exec, hipGraphNode_t node, size_
  * reference updaters read every node back with hipGraphKernelNodeGetParams
  * (causal_attention.hip.cpp:981,1009; rope.hip.cpp:215), which is what is
  * done here for nodes without a record.  Returns the number of records
- * held. */
+ * held.  (The paged and 4-bit calls below are not recorded: what changes between
+ * their replays lives in device memory, so there is nothing to patch.) */
 size_t attn_graph_node_records(void);
 
 /* No single counterpart in the reference: launch_rope_and_store_kv(q, k, v,

@@ -157,8 +157,8 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 def _stream(stream) -> Optional[int]:
     if stream is None:
-        if _raw_stream is not None and torch.cuda.is_initialized():
-            return _raw_stream(torch.cuda.current_device())
+        if _raw_stream is not None:
+            return _raw_stream(torch.cuda.current_device())  # initialises CUDA if need be
         return torch.cuda.current_stream().cuda_stream
     if isinstance(stream, int):
         return stream
@@ -321,18 +321,48 @@ def decode_out_proj(q, k_cache, v_cache, attn_out, partial_out, partial_max, par
         nodes[:] = [an.value, mn.value]
 
 
+_INT32 = torch.int32
+
+
+def _ints(x, what) -> Optional[int]:
+    """Address of an int32 array; a tensor of another type or order is refused (torch
+    makes int64 by itself, whose halves would pass for page numbers and lengths)."""
+    if x is None or isinstance(x, int):
+        return x
+    if x.dtype is _INT32 and x.is_contiguous():
+        return x.data_ptr()
+    raise AttnError(f"{what} must be a contiguous int32 tensor, got {x.dtype}")
+
+
+def _call(fn, what, on, stream, *args):
+    """fn(*args, stream) on the device of the tensor `on` (an address: the current one)."""
+    if isinstance(on, int):
+        rc = fn(*args, _stream(stream))
+    else:
+        device = torch.cuda.current_device()
+        if on.get_device() != device:
+            with torch.cuda.device(on.device):
+                rc = fn(*args, _stream(stream))
+        elif stream is None and _raw_stream is not None:
+            rc = fn(*args, _raw_stream(device))
+        else:
+            rc = fn(*args, _stream(stream))
+    if rc != 0:
+        _check(rc, what)
+
+
 def paged_rope_store_kv(q, k, v, k_pages, v_pages, cos, sin, page_table, positions, num_tokens,
                         num_seqs, max_pages, num_pages, page_size, max_seq_len, num_heads,
                         num_kv_heads, head_dim, q_stride=0, k_stride=0, apply_rotation=True,
                         q_out=None, seq_ids=None, stream=None):
     """rope_store_kv into the pages of a paged cache, for any set of tokens: token t
     at positions[t] of sequence seq_ids[t] (None: sequence t)."""
-    rc = lib().attn_paged_rope_store_kv(
-        _ptr(q), _ptr(k), _ptr(v), _ptr(q_out), _ptr(k_pages), _ptr(v_pages), _ptr(cos),
-        _ptr(sin), _ptr(page_table), _ptr(seq_ids), _ptr(positions), num_tokens, num_seqs,
-        max_pages, num_pages, page_size, max_seq_len, num_heads, num_kv_heads, head_dim,
-        q_stride, k_stride, 1 if apply_rotation else 0, _stream(stream))
-    _check(rc, "attn_paged_rope_store_kv")
+    _call(lib().attn_paged_rope_store_kv, "attn_paged_rope_store_kv", k_pages, stream, _ptr(q),
+          _ptr(k), _ptr(v), _ptr(q_out), _ptr(k_pages), _ptr(v_pages), _ptr(cos), _ptr(sin),
+          _ints(page_table, "page_table"), _ints(seq_ids, "seq_ids"),
+          _ints(positions, "positions"), num_tokens, num_seqs, max_pages, num_pages, page_size,
+          max_seq_len, num_heads, num_kv_heads, head_dim, q_stride, k_stride,
+          1 if apply_rotation else 0)
 
 
 def paged_decode_workspace(num_seqs, num_heads, num_kv_heads, head_dim, device="cuda"):
@@ -345,11 +375,10 @@ def paged_decode(q, k_pages, v_pages, out, page_table, kv_lens, num_seqs, max_pa
                  page_size, num_heads, num_kv_heads, head_dim, workspace, q_stride=0,
                  stream=None):
     """Decode attention of one new token per sequence over its pages."""
-    rc = lib().attn_paged_decode(_ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(out),
-                                 _ptr(page_table), _ptr(kv_lens), num_seqs, max_pages, num_pages,
-                                 page_size, num_heads, num_kv_heads, head_dim, q_stride,
-                                 _ptr(workspace), _stream(stream))
-    _check(rc, "attn_paged_decode")
+    _call(lib().attn_paged_decode, "attn_paged_decode", out, stream, _ptr(q), _ptr(k_pages),
+          _ptr(v_pages), _ptr(out), _ints(page_table, "page_table"), _ints(kv_lens, "kv_lens"),
+          num_seqs, max_pages, num_pages, page_size, num_heads, num_kv_heads, head_dim, q_stride,
+          _ptr(workspace))
 
 
 def pages_workspace(num_seqs, num_pages, device="cuda"):
@@ -360,72 +389,69 @@ def pages_workspace(num_seqs, num_pages, device="cuda"):
 
 def pages_copy(pool, num_planes, page_elems, src, dst, n, num_pages, plane_stride=0, stream=None):
     """Pages src[i] -> dst[i] in every plane of the pool."""
-    rc = lib().attn_pages_copy(_ptr(pool), num_planes, plane_stride, page_elems, _ptr(src),
-                               _ptr(dst), n, num_pages, _stream(stream))
-    _check(rc, "attn_pages_copy")
+    _call(lib().attn_pages_copy, "attn_pages_copy", pool, stream, _ptr(pool), num_planes,
+          plane_stride, page_elems, _ints(src, "src"), _ints(dst, "dst"), n, num_pages)
 
 
 def pages_free(page_table, seq_lens, ref_counts, num_seqs, max_pages, num_pages, page_size,
                keep_lens=None, stream=None):
     """Cuts every sequence to keep_lens[b] tokens (None: 0)."""
-    rc = lib().attn_pages_free(_ptr(page_table), _ptr(seq_lens), _ptr(keep_lens),
-                               _ptr(ref_counts), num_seqs, max_pages, num_pages, page_size,
-                               _stream(stream))
-    _check(rc, "attn_pages_free")
+    _call(lib().attn_pages_free, "attn_pages_free", page_table, stream,
+          _ints(page_table, "page_table"), _ints(seq_lens, "seq_lens"),
+          _ints(keep_lens, "keep_lens"), _ints(ref_counts, "ref_counts"), num_seqs, max_pages,
+          num_pages, page_size)
 
 
 def pages_fork(src_table, src_lens, dst_table, dst_lens, parents, ref_counts, num_src, num_dst,
                max_pages, num_pages, page_size, stream=None):
     """Row i of the destination table shares the pages of source row parents[i]."""
-    rc = lib().attn_pages_fork(_ptr(src_table), _ptr(src_lens), _ptr(dst_table), _ptr(dst_lens),
-                               _ptr(parents), _ptr(ref_counts), num_src, num_dst, max_pages,
-                               num_pages, page_size, _stream(stream))
-    _check(rc, "attn_pages_fork")
+    _call(lib().attn_pages_fork, "attn_pages_fork", dst_table, stream,
+          _ints(src_table, "src_table"), _ints(src_lens, "src_lens"),
+          _ints(dst_table, "dst_table"), _ints(dst_lens, "dst_lens"), _ints(parents, "parents"),
+          _ints(ref_counts, "ref_counts"), num_src, num_dst, max_pages, num_pages, page_size)
 
 
 def pages_grow(pool, num_planes, page_elems, page_table, seq_lens, grow, ref_counts, status,
                num_seqs, max_pages, num_pages, page_size, workspace, plane_stride=0,
                stream=None):
     """Sequence b grows by grow[b] tokens: new pages, and a copy of a shared last one."""
-    rc = lib().attn_pages_grow(_ptr(pool), num_planes, plane_stride, page_elems,
-                               _ptr(page_table), _ptr(seq_lens), _ptr(grow), _ptr(ref_counts),
-                               _ptr(status), num_seqs, max_pages, num_pages, page_size,
-                               _ptr(workspace), _stream(stream))
-    _check(rc, "attn_pages_grow")
+    _call(lib().attn_pages_grow, "attn_pages_grow", pool, stream, _ptr(pool), num_planes,
+          plane_stride, page_elems, _ints(page_table, "page_table"),
+          _ints(seq_lens, "seq_lens"), _ints(grow, "grow"), _ints(ref_counts, "ref_counts"),
+          _ints(status, "status"), num_seqs, max_pages, num_pages, page_size, _ptr(workspace))
 
 
 def pages_compact(pool, num_planes, page_elems, page_table, seq_lens, ref_counts, page_table_out,
                   ref_counts_out, num_used, num_seqs, max_pages, num_pages, page_size, workspace,
                   plane_stride=0, stream=None):
     """Moves the used pages to the front of the pool."""
-    rc = lib().attn_pages_compact(_ptr(pool), num_planes, plane_stride, page_elems,
-                                  _ptr(page_table), _ptr(seq_lens), _ptr(ref_counts),
-                                  _ptr(page_table_out), _ptr(ref_counts_out), _ptr(num_used),
-                                  num_seqs, max_pages, num_pages, page_size, _ptr(workspace),
-                                  _stream(stream))
-    _check(rc, "attn_pages_compact")
+    _call(lib().attn_pages_compact, "attn_pages_compact", pool, stream, _ptr(pool), num_planes,
+          plane_stride, page_elems, _ints(page_table, "page_table"),
+          _ints(seq_lens, "seq_lens"), _ints(ref_counts, "ref_counts"),
+          _ints(page_table_out, "page_table_out"), _ints(ref_counts_out, "ref_counts_out"),
+          _ints(num_used, "num_used"), num_seqs, max_pages, num_pages, page_size, _ptr(workspace))
 
 
 def w4_pack(w, out_dim, in_dim, group_size, stream=None):
     """4-bit codes and group scales of fp16 weights [out_dim][in_dim] (a tensor, or a
     view such as ModelWeights.qkv): (packed, scales) for w4_matvec."""
+    if w.dtype is not torch.float16 or not w.is_contiguous() or w.numel() < out_dim * in_dim:
+        raise AttnError(f"w4_pack needs {out_dim} x {in_dim} contiguous fp16 weights")
     packed = torch.empty(int(lib().attn_w4_weight_bytes(out_dim, in_dim)), dtype=torch.uint8,
                          device=w.device)
     scales = torch.empty(int(lib().attn_w4_scale_count(out_dim, in_dim, group_size)),
                          dtype=torch.float16, device=w.device)
-    rc = lib().attn_w4_pack(_ptr(w), _ptr(packed), _ptr(scales), out_dim, in_dim, group_size,
-                            _stream(stream))
-    _check(rc, "attn_w4_pack")
+    _call(lib().attn_w4_pack, "attn_w4_pack", w, stream, _ptr(w), _ptr(packed), _ptr(scales),
+          out_dim, in_dim, group_size)
     return packed, scales
 
 
 def w4_matvec(x, y, packed, scales, num_tokens, in_dim, out_dim, group_size, residual=None,
               x_stride=0, y_stride=0, stream=None):
     """y[t] = W x[t] (+ residual[t]) with 4-bit weights."""
-    rc = lib().attn_w4_matvec(_ptr(x), _ptr(y), _ptr(packed), _ptr(scales), _ptr(residual),
-                              num_tokens, in_dim, out_dim, group_size, x_stride, y_stride,
-                              _stream(stream))
-    _check(rc, "attn_w4_matvec")
+    _call(lib().attn_w4_matvec, "attn_w4_matvec", y, stream, _ptr(x), _ptr(y), _ptr(packed),
+          _ptr(scales), _ptr(residual), num_tokens, in_dim, out_dim, group_size, x_stride,
+          y_stride)
 
 
 def decode_plan(kv_len, num_heads, num_kv_heads, head_dim, kv_stride=0, q=None, k=None,

@@ -130,6 +130,23 @@ def test_w4_refusals(attn):
     assert lib.attn_w4_scale_count(17, 129, 0) == 0
 
 
+def test_wrappers_refuse_other_integers(attn):
+    """Page numbers and lengths in 64 bits, or in another order, never reach the library."""
+    import torch
+    good = torch.zeros(4, 4, dtype=torch.int32)
+    for bad in (good.long(), good.float(), good.t()[1:], good[:, ::2]):
+        with pytest.raises(attn.AttnError, match="kv_lens must be a contiguous int32"):
+            attn.paged_decode(P, P, P, P, good, bad, 4, 4, 8, 16, 4, 2, 64, P)
+        with pytest.raises(attn.AttnError, match="page_table must be"):
+            attn.pages_free(bad, good, good, 4, 4, 8, 16)
+        with pytest.raises(attn.AttnError, match="positions must be"):
+            attn.paged_rope_store_kv(P, P, P, P, P, P, P, good, bad, 4, 4, 4, 8, 16, 9, 4, 2, 64)
+    for w in (torch.zeros(4, 64), torch.zeros(64, 4, dtype=torch.float16).t(),
+              torch.zeros(4, 63, dtype=torch.float16)):
+        with pytest.raises(attn.AttnError, match="4 x 64 contiguous fp16"):
+            attn.w4_pack(w, 4, 64, 32)
+
+
 @pytest.mark.parametrize("N,K", [(1, 1), (16, 128), (35, 300)])
 def test_reference_words_hold_every_code(N, K):
     codes = np.random.default_rng(N).integers(0, 16, (N, K))
