@@ -11,9 +11,14 @@
 // Nothing synchronises with the host, so the calls can be captured; a pool that runs
 // short is reported in a status word and leaves the state as it was.
 //
-// Planning kernels are one workgroup of 1024 threads (a few microseconds up to some
-// ten thousand pages); pages move in a second launch over the whole GPU.  Bound by
-// HBM for the pages that move, by launches and the plan's chain of loads otherwise.
+// Planning kernels are one workgroup of 1024 threads, 4096 pages a round: the order of
+// the free pages is a prefix sum, which ballots give within a workgroup without a second
+// launch.  Pages move in a launch of their own over the whole GPU, 16 KiB a workgroup and
+// turn.  Bound by HBM for the pages that move, by launches and the plan's chain of loads
+// (length -> page -> count -> free pages) otherwise.  Measured (traced, pages of 16 rows of
+// 512 values in 72 planes, 4096 pages): 256 forks that copy 208 pages: free 3.5 us, fork 3.8,
+// plan 6.6, copy 85.5 (5.7 TB/s); a compaction that moves 283 pages: plan 5.0, copy 126
+// (5.3 TB/s); four forks: 1.4, 2.0, 4.9 and 2.6.
 #include "paged_internal.hpp"
 #include "../../include/attn_mi355x.h"
 

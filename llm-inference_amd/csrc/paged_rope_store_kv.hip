@@ -16,7 +16,9 @@
 // Bound by HBM, and for small batches by the chain position -> page -> row.  One lane
 // owns 8 rotation pairs of a head (two 16-byte loads and stores), as in
 // rope_store_kv_vec; every lane looks its token's page up by itself (the loads of a
-// token's lanes hit one cache line), which needs no barrier.
+// token's lanes hit one cache line), which needs no barrier.  Measured (16/4 heads of
+// 128, traced): 2000 tokens 6.4 us for 25.1 MB (3.9 TB/s, one round of loads), 64 tokens
+// 2.9 us.
 #include "paged_internal.hpp"
 #include "../../include/attn_mi355x.h"
 

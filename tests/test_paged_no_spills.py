@@ -1,0 +1,25 @@
+"""Registers of the paged decode and of the 4-bit products, from the compiler's own report:
+both keep two units or tiles in flight, and a kernel that spills waits for its own stores."""
+import pathlib
+import re
+import subprocess
+
+import pytest
+
+CSRC = pathlib.Path(__file__).resolve().parents[1] / "llm-inference_amd" / "csrc"
+
+
+@pytest.mark.parametrize("source,least", [("paged_decode", 24), ("w4_matvec", 14)])
+def test_kernels_do_not_spill(tmp_path, source, least):
+    # the build's own command line for this file
+    out = subprocess.run(["make", "-C", str(CSRC), "-n", "-B", f"../lib/obj/{source}.o"],
+                         capture_output=True, text=True, check=True).stdout
+    line = next(x for x in out.splitlines() if f"-c {source}.hip" in x)
+    line = re.sub(r"-o \S+", f"-o {tmp_path / 'x.o'}", line)
+    r = subprocess.run(line + " -Rpass-analysis=kernel-resource-usage", shell=True, cwd=CSRC,
+                       capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+    names = re.findall(r"Function Name: (\S+)", r.stderr)
+    spills = [int(x) for x in re.findall(r"VGPRs Spill: (\d+)", r.stderr)]
+    assert len(names) == len(spills) >= least, r.stderr[-2000:]
+    assert not any(spills), dict(zip(names, spills))
