@@ -63,6 +63,19 @@ struct PagedDecodeArgs {
     uint32_t pad_;
 };
 
+// A score in the log2 domain, rounded before anything is taken from it, and 2^(x - m +
+// bits): x - m is then never above 0, however large the scores are.  (One multiply-add of
+// score, scale and -m is off by half a step of m instead, 32 at scores of 10^9, and the
+// weight overflows.)
+__device__ __forceinline__ float scaled_score(float dot, float scale) {
+#pragma clang fp contract(off)
+    return dot * scale;
+}
+__device__ __forceinline__ float weight(float x, float m, float bits) {
+#pragma clang fp contract(off)
+    return fast_exp2((x - m) + bits);
+}
+
 // Head dims other than 64 and 128, unaligned tensors: one workgroup per sequence and
 // query head, tiles of 256 keys, one score per thread, then a dim per
 // thread; fp32 throughout.
@@ -95,14 +108,14 @@ __global__ __launch_bounds__(kTile) void paged_decode_generic(PagedDecodeArgs a)
                 dot = 0.f;
                 for (uint32_t d = 0; d < D; ++d) dot += s_q[d] * (float)kr[d];
             }
-            s = dot * a.scale_log2;
+            s = scaled_score(dot, a.scale_log2);
         }
         const float wm = wave_max(s);
         if ((tid & 63u) == 0) s_red[0][wave] = wm;
         __syncthreads();
         const float m_new = fmaxf(fmaxf(fmaxf(s_red[0][0], s_red[0][1]),
                                         fmaxf(s_red[0][2], s_red[0][3])), m_run);
-        const float p = j < len ? fast_exp2(s - m_new) : 0.f;
+        const float p = j < len ? weight(s, m_new, 0.f) : 0.f;
         s_p[tid] = p;
         const float wl = wave_sum(p);
         if ((tid & 63u) == 0) s_red[1][wave] = wl;
@@ -362,17 +375,18 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_split(PagedSplitArgs
                             x.v[r] = VRow{};
                         }
                 }
-                float mx = st[0][0];
+                float x_log2[8], mx = -INFINITY;
 #pragma unroll
-                for (int r = 1; r < 8; ++r) mx = fmaxf(mx, st[r >> 2][r & 3]);
-                mx = max_xor<32>(max_xor<16>(mx)) * a.scale_log2;
+                for (int r = 0; r < 8; ++r) {
+                    x_log2[r] = scaled_score(st[r >> 2][r & 3], a.scale_log2);
+                    mx = fmaxf(mx, x_log2[r]);
+                }
+                mx = max_xor<32>(max_xor<16>(mx));
                 const float m_new = fmaxf(m_run, mx);
                 const float alpha = fast_exp2(m_run - m_new);
-                const float shift = kWeightBits - m_new;
                 f16x8 p;
 #pragma unroll
-                for (int r = 0; r < 8; ++r)
-                    p[r] = (f16)fast_exp2(__builtin_fmaf(st[r >> 2][r & 3], a.scale_log2, shift));
+                for (int r = 0; r < 8; ++r) p[r] = (f16)weight(x_log2[r], m_new, kWeightBits);
                 const f16x2 one = {(f16)1.0f, (f16)1.0f};
                 float sum = 0.f;
 #pragma unroll

@@ -140,6 +140,26 @@ def test_rising_scores(attn, gpu, D):
     c.check(c.got())
 
 
+@pytest.mark.parametrize("size", [300.0, 3000.0, 30000.0])
+@pytest.mark.parametrize("D", [128, 64])
+def test_scores_far_past_the_steps_of_fp32(attn, gpu, form, D, size):
+    """Scores of 10^6 to 10^11, whose neighbours in fp32 are up to 8192 apart: the one key
+    that points along the query has all the weight, the others point away."""
+    c = Case(attn, gpu, [200], 16, 8, 2, D, seed=17, columns=columns_of(form, 16, 200))
+    rng = np.random.default_rng(18)
+    sign = rng.choice([-1.0, 1.0], (c.Hkv, D))
+    c.q[0] = np.repeat(size * sign, c.Hq // c.Hkv, axis=0).ravel()
+    rows = c.lay.rows(0)
+    # sums of odd values, so that products with the scale are not exact in fp32
+    c.k[rows] = -sign * (size * rng.uniform(0.5, 1.0, (len(rows), c.Hkv, D)))
+    c.k[rows[77]] = sign * (size * rng.uniform(0.5, 1.0, (c.Hkv, D)))
+    c.upload()
+    c.call()
+    got = c.got()[0]
+    exp = np.repeat(c.v[rows[77]], c.Hq // c.Hkv, axis=0)
+    assert np.array_equal(got.view(np.uint16), exp.view(np.uint16))
+
+
 @pytest.mark.parametrize("D", [128, 64])
 def test_many_small_weights_keep_their_sum(attn, gpu, D):
     """One key whose weight is 2^17 times the others': alone they would vanish in fp16,
