@@ -17,8 +17,9 @@
 // MB in 26.7 us, 5.1 TB/s), by latency for few rows (2048 x 2048: 4.0 us).  For a batch
 // the workgroups' reads of x bound it: each reads its tokens' whole rows from the L2, at
 // about 9 ns a KiB and CU (33 tokens, 2048 x 11008, groups of 32: 14.4 us, of which the
-// weights' 11.3 MB would take 2.7).  Sharing the columns between workgroups would divide
-// those reads, but takes a workspace and a second kernel for the sums.
+// weights' 11.3 MB would take 2.7).  Many rows share those reads between the waves of a
+// workgroup; for few rows, sharing the columns between workgroups would divide them, but
+// takes a workspace and a second kernel for the sums.
 #include "attn_internal.hpp"
 #include "../../include/attn_mi355x.h"
 
@@ -71,8 +72,8 @@ __device__ __forceinline__ f16x8 w4_values(uint32_t word, const W4Consts& k) {
     return f16x8{v0[0], v0[1], v1[0], v1[1], v2[0], v2[1], v3[0], v3[1]};
 }
 
-// 16 bytes of codes per lane.  Without the non-temporal hint: 64 tokens, 12000 x 12000
-// 50 us against 60 with it, one token, 128256 x 2048 (HBM-cold) level.
+// 16 bytes of codes per lane.  Without the non-temporal hint: 16 tokens, 12000 x 12000 22.8
+// us against 28.1 with it, one token, 128256 x 2048 (HBM-cold) level.
 __device__ __forceinline__ u32x4 w4_load(BufRsrc rows, uint32_t byte_off) {
     return __builtin_bit_cast(u32x4,
                               __builtin_amdgcn_raw_buffer_load_b128(rows, (int)byte_off, 0, 0));
@@ -188,17 +189,17 @@ __device__ __forceinline__ f16x4 w4_step_scale(u32x2 mine) {
     return __builtin_bit_cast(f16x4, v);
 }
 
-// Any number of tokens: R row tiles x TT tiles of 16 tokens a wave.  SPS: steps of 32
-// columns that share a scale at least (4: the group is a multiple of 128; 2: of 64; 1).
-// The products of a scale's columns are summed by the MFMAs from zero, then scaled and
-// added in fp32, so no product is rounded.
-template <int R, int TT, int SPS, bool VEC>
+// Few rows: R row tiles x 16 tokens a wave, the waves of a row tile split the columns, each
+// with its own x.  SPS: steps of 32 columns that share a scale at least (4: the group is a
+// multiple of 128; 2: of 64; 1).  The products of a scale's columns are summed by the MFMAs
+// from zero, then scaled and added in fp32, so no product is rounded.
+template <int R, int SPS, bool VEC>
 __global__ __launch_bounds__(64 * kW4Waves) void w4_matvec(W4Args a) {
     constexpr int kDepth = VEC ? 2 : 1;  // column tiles in flight
-    // a wave's x tile (16 tokens x 128 columns each), then the waves' sums
+    // a wave's x tile (16 tokens x 128 columns), then the waves' sums
     union Shared {
-        f16x8 x[kW4Waves][TT][256];
-        float part[kW4Waves][16 * TT][16 * R + 1];
+        f16x8 x[kW4Waves][256];
+        float part[kW4Waves][16][16 * R + 1];
     };
     __shared__ __attribute__((aligned(16))) Shared s_mem;
     const uint32_t lane = threadIdx.x & 63u;
@@ -206,24 +207,20 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matvec(W4Args a) {
     const uint32_t n = lane & 15u, gq = lane >> 4;
     const uint32_t rt = (blockIdx.x * kW4Waves + wave) / a.split * R;
     const uint32_t first = wave & (a.split - 1u);
-    const uint32_t t0 = blockIdx.y * 16u * TT;
+    const uint32_t t0 = blockIdx.y * 16u;
+    const uint32_t live = min(a.tokens - t0, 16u);
     const W4Consts consts;
-    const uint32_t live = min(a.tokens - t0, 16u * (uint32_t)TT);
-    f32x4 acc[R][TT];
+    f32x4 acc[R];
 #pragma unroll
-    for (int q = 0; q < R; ++q)
-#pragma unroll
-        for (int tt = 0; tt < TT; ++tt) acc[q][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int q = 0; q < R; ++q) acc[q] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (rt < a.row_tiles && a.col_tiles > 0) {
-        // row tiles past the last one read nothing
-        const uint32_t tile_bytes = a.col_tiles * 1024u;
         BufRsrc rw[R];
         const f16* sc[R];
         const uint64_t sc_stride = (uint64_t)a.row_tiles * 16u;
 #pragma unroll
-        for (int q = 0; q < R; ++q) {
+        for (int q = 0; q < R; ++q) {  // row tiles past the last one repeat it and are not stored
             const uint32_t r = min(rt + q, a.row_tiles - 1u);
-            rw[q] = make_rsrc(a.w + (uint64_t)r * a.col_tiles * 256u, tile_bytes);
+            rw[q] = make_rsrc(a.w + (uint64_t)r * a.col_tiles * 256u, a.col_tiles * 1024u);
             sc[q] = a.scales + r * 16u + 4u * gq;
         }
         const f16* const xb = a.x + (uint64_t)t0 * a.x_stride;
@@ -232,15 +229,13 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matvec(W4Args a) {
         // bytes, as the MFMA operand wants it, took the load pipe twice as long), and turned
         // in LDS: row r's 16-byte chunk i lies at chunk i ^ r, so that the 16 rows of an
         // operand read cover all banks.
-        uint64_t x_at[TT][4];  // elements; tokens past the last repeat it: nothing of theirs is stored
+        uint64_t x_at[4];  // elements; tokens past the last repeat it: nothing of theirs is stored
 #pragma unroll
-        for (int tt = 0; tt < TT; ++tt)
-#pragma unroll
-            for (uint32_t j = 0; j < 4; ++j)
-                x_at[tt][j] = min(16u * tt + 4u * j + gq, live - 1u) * a.x_stride + 8u * n;
+        for (uint32_t j = 0; j < 4; ++j)
+            x_at[j] = min(4u * j + gq, live - 1u) * a.x_stride + 8u * n;
         struct Stage {
             u32x4 w[R];
-            f16x8 x[TT][4];
+            f16x8 x[4];
             u32x2 scale[R];  // of step n % 4, rows 4 gq ..
         } st[kDepth];
         auto load = [&](uint32_t c, Stage& z) {
@@ -252,48 +247,35 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matvec(W4Args a) {
             }
             const uint32_t k = 128u * c + 8u * n;
 #pragma unroll
-            for (int tt = 0; tt < TT; ++tt)
+            for (uint32_t j = 0; j < 4; ++j) {
+                if constexpr (VEC) {
+                    z.x[j] = buf_ld16(rx, k < a.cols ? 2u * ((uint32_t)x_at[j] + 128u * c) : kDead);
+                } else {
 #pragma unroll
-                for (uint32_t j = 0; j < 4; ++j) {
-                    if constexpr (VEC) {
-                        z.x[tt][j] = buf_ld16(
-                            rx, k < a.cols ? 2u * ((uint32_t)x_at[tt][j] + 128u * c) : kDead);
-                    } else {
-#pragma unroll
-                        for (uint32_t e = 0; e < 8; ++e)
-                            z.x[tt][j][e] =
-                                k + e < a.cols ? xb[x_at[tt][j] + 128u * c + e] : (f16)0.f;
-                    }
+                    for (uint32_t e = 0; e < 8; ++e)
+                        z.x[j][e] = k + e < a.cols ? xb[x_at[j] + 128u * c + e] : (f16)0.f;
                 }
+            }
         };
         auto compute = [&](const Stage& z) {
 #pragma unroll
-            for (int tt = 0; tt < TT; ++tt)
-#pragma unroll
-                for (uint32_t j = 0; j < 4; ++j) {
-                    const uint32_t r = 4u * j + gq;
-                    s_mem.x[wave][tt][16u * r + (n ^ r)] = z.x[tt][j];
-                }
-            f32x4 part[R][TT];
+            for (uint32_t j = 0; j < 4; ++j) {
+                const uint32_t r = 4u * j + gq;
+                s_mem.x[wave][16u * r + (n ^ r)] = z.x[j];
+            }
+            f32x4 part[R];
             auto step = [&]<int s>() {
-                f16x8 xv[TT];
-#pragma unroll
-                for (int tt = 0; tt < TT; ++tt)
-                    xv[tt] = s_mem.x[wave][tt][16u * n + ((4u * s + gq) ^ n)];
+                const f16x8 xv = s_mem.x[wave][16u * n + ((4u * s + gq) ^ n)];
 #pragma unroll
                 for (int q = 0; q < R; ++q) {
                     const f16x8 wv = w4_values(z.w[q][s], consts);
                     const f16x4 scale = w4_step_scale<s>(z.scale[q]);
+                    if (s % SPS == 0) part[q] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    part[q] = mfma16(wv, xv, part[q]);
+                    if (s % SPS == SPS - 1)
 #pragma unroll
-                    for (int tt = 0; tt < TT; ++tt) {
-                        if (s % SPS == 0) part[q][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
-                        part[q][tt] = mfma16(wv, xv[tt], part[q][tt]);
-                        if (s % SPS == SPS - 1)
-#pragma unroll
-                            for (int r = 0; r < 4; ++r)
-                                acc[q][tt][r] =
-                                    __builtin_fmaf((float)scale[r], part[q][tt][r], acc[q][tt][r]);
-                    }
+                        for (int r = 0; r < 4; ++r)
+                            acc[q][r] = __builtin_fmaf((float)scale[r], part[q][r], acc[q][r]);
                 }
             };
             step.template operator()<0>();
@@ -316,32 +298,171 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matvec(W4Args a) {
 #pragma unroll
     for (int q = 0; q < R; ++q)
 #pragma unroll
-        for (int tt = 0; tt < TT; ++tt)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                s_mem.part[wave][16 * tt + n][16 * q + 4u * gq + r] = acc[q][tt][r];
+        for (int r = 0; r < 4; ++r) s_mem.part[wave][n][16 * q + 4u * gq + r] = acc[q][r];
     __syncthreads();
-    w4_store<16 * TT, R>(a, s_mem.part, t0, live);
+    w4_store<16, R>(a, s_mem.part, t0, live);
 }
 
-template <int R, int TT, int SPS>
+template <int R, int SPS>
 hipError_t launch_w4(const W4Args& a, bool vec, hipStream_t stream) {
     const uint32_t tiles = kW4Waves / a.split * R;
-    const dim3 grid((a.row_tiles + tiles - 1u) / tiles, (a.tokens + 16u * TT - 1u) / (16u * TT));
+    const dim3 grid((a.row_tiles + tiles - 1u) / tiles, (a.tokens + 15u) / 16u);
     if (vec)
-        hipLaunchKernelGGL((w4_matvec<R, TT, SPS, true>), grid, dim3(64 * kW4Waves), 0, stream, a);
-    else if constexpr (TT == 1)  // two token tiles of element-wise loads spill
-        hipLaunchKernelGGL((w4_matvec<R, TT, SPS, false>), grid, dim3(64 * kW4Waves), 0, stream, a);
+        hipLaunchKernelGGL((w4_matvec<R, SPS, true>), grid, dim3(64 * kW4Waves), 0, stream, a);
     else
-        return hipErrorInvalidValue;
+        hipLaunchKernelGGL((w4_matvec<R, SPS, false>), grid, dim3(64 * kW4Waves), 0, stream, a);
     return hipGetLastError();
 }
 
-template <int R, int TT>
+template <int R>
 hipError_t launch_w4(const W4Args& a, bool vec, hipStream_t stream) {
-    if (a.group % 128 == 0) return launch_w4<R, TT, 4>(a, vec, stream);
-    if (a.group % 64 == 0) return launch_w4<R, TT, 2>(a, vec, stream);
-    return launch_w4<R, TT, 1>(a, vec, stream);
+    if (a.group % 128 == 0) return launch_w4<R, 4>(a, vec, stream);
+    if (a.group % 64 == 0) return launch_w4<R, 2>(a, vec, stream);
+    return launch_w4<R, 1>(a, vec, stream);
+}
+
+// Many rows and tokens: RW of the eight waves take row tiles of their own (R each) and share
+// x, so that a workgroup reads x once for 16 R RW rows; the 8 / RW groups of waves split the
+// columns.  x goes through two LDS tiles in turn: each wave of a group loads its part of the
+// next tile into registers, and one barrier a column tile parts the writes from the reads.
+// Tiles past the last column are zeros through the range checks, so every wave runs the same
+// number of rounds.
+template <int R, int TT, int RW, int SPS>
+__global__ __launch_bounds__(64 * kW4Waves) void w4_matmul(W4Args a) {
+    constexpr uint32_t kGroups = kW4Waves / RW;
+    constexpr int kLoads = 4 * TT / RW;  // of a wave for a tile of x
+    static_assert(kLoads * RW == 4 * TT);
+    constexpr uint32_t kRows = 16 * R * RW;
+    union Shared {
+        f16x8 x[2][kGroups][TT][256];
+        float part[kGroups][16 * TT][kRows + 1];
+    };
+    __shared__ __attribute__((aligned(16))) Shared s_mem;
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t n = lane & 15u, gq = lane >> 4;
+    const uint32_t kg = wave / RW, rg = wave % RW;
+    const uint32_t rt = (blockIdx.x * RW + rg) * R;
+    const uint32_t t0 = blockIdx.y * 16u * TT;
+    const uint32_t live = min(a.tokens - t0, 16u * (uint32_t)TT);
+    const W4Consts consts;
+    BufRsrc rw[R];
+    const f16* sc[R];
+    const uint64_t sc_stride = (uint64_t)a.row_tiles * 16u;
+#pragma unroll
+    for (int q = 0; q < R; ++q) {  // row tiles past the last one repeat it and are not stored
+        const uint32_t r = min(rt + q, a.row_tiles - 1u);
+        rw[q] = make_rsrc(a.w + (uint64_t)r * a.col_tiles * 256u, a.col_tiles * 1024u);
+        sc[q] = a.scales + r * 16u + 4u * gq;
+    }
+    const BufRsrc rx = make_rsrc(a.x + (uint64_t)t0 * a.x_stride,
+                                 (uint32_t)(((live - 1u) * a.x_stride + a.cols) * 2u));
+    // load i of this wave: rows 4 (rg + RW i) .. + 3 of the token tiles, 256 bytes each
+    uint32_t x_at[kLoads], x_to[kLoads];
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+        const uint32_t q = rg + RW * i, r = 4u * (q & 3u) + gq;
+        x_at[i] = 2u * (uint32_t)(min(4u * q + gq, live - 1u) * a.x_stride + 8u * n);
+        x_to[i] = (q >> 2) * 256u + 16u * r + (n ^ r);
+    }
+    struct Weights {
+        u32x4 w[R];
+        u32x2 scale[R];  // of step n % 4, rows 4 gq ..
+    };
+    f16x8 xr[kLoads];
+    auto load_x = [&](uint32_t c) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i)
+            xr[i] = buf_ld16(rx, 128u * c + 8u * n < a.cols ? x_at[i] + 256u * c : kDead);
+    };
+    auto load_w = [&](uint32_t c, Weights& z) {
+        const uint64_t at = w4_group(a, min(128u * c + 32u * (n & 3u), a.cols - 1u)) * sc_stride;
+#pragma unroll
+        for (int q = 0; q < R; ++q) {
+            z.w[q] = w4_load(rw[q], c * 1024u + 16u * lane);
+            z.scale[q] = *reinterpret_cast<const u32x2*>(sc[q] + at);
+        }
+    };
+    f32x4 acc[R][TT];
+#pragma unroll
+    for (int q = 0; q < R; ++q)
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) acc[q][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto compute = [&](const f16x8 (*x)[256], const Weights& z) {
+        f32x4 part[R][TT];
+        auto step = [&]<int s>() {
+            f16x8 xv[TT];
+#pragma unroll
+            for (int tt = 0; tt < TT; ++tt) xv[tt] = x[tt][16u * n + ((4u * s + gq) ^ n)];
+#pragma unroll
+            for (int q = 0; q < R; ++q) {
+                const f16x8 wv = w4_values(z.w[q][s], consts);
+                const f16x4 scale = w4_step_scale<s>(z.scale[q]);
+#pragma unroll
+                for (int tt = 0; tt < TT; ++tt) {
+                    if (s % SPS == 0) part[q][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    part[q][tt] = mfma16(wv, xv[tt], part[q][tt]);
+                    if (s % SPS == SPS - 1)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            acc[q][tt][r] =
+                                __builtin_fmaf((float)scale[r], part[q][tt][r], acc[q][tt][r]);
+                }
+            }
+        };
+        step.template operator()<0>();
+        step.template operator()<1>();
+        step.template operator()<2>();
+        step.template operator()<3>();
+    };
+    Weights wa, wb;
+    load_w(kg, wa);
+    load_x(kg);
+    auto round = [&](uint32_t c, uint32_t buf, const Weights& now, Weights& next) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) (&s_mem.x[buf][kg][0][0])[x_to[i]] = xr[i];
+        __syncthreads();
+        load_w(c + kGroups, next);
+        load_x(c + kGroups);
+        compute(s_mem.x[buf][kg], now);
+    };
+    for (uint32_t c = kg; c < a.col_tiles + kg; c += 2u * kGroups) {
+        round(c, 0u, wa, wb);
+        round(c + kGroups, 1u, wb, wa);
+    }
+    __syncthreads();  // x is read
+#pragma unroll
+    for (int q = 0; q < R; ++q)
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                s_mem.part[kg][16 * tt + n][16u * (R * rg + q) + 4u * gq + r] = acc[q][tt][r];
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < live * kRows; i += 64u * kW4Waves) {
+        const uint32_t t = i / kRows, r = i % kRows, row = blockIdx.x * kRows + r;
+        if (row >= a.rows) continue;
+        float sum = 0.f;
+#pragma unroll
+        for (uint32_t x = 0; x < kGroups; ++x) sum += s_mem.part[x][t][r];
+        const uint64_t at = (uint64_t)(t0 + t) * a.y_stride + row;
+        if (a.residual) sum += (float)a.residual[at];
+        a.y[at] = (f16)sum;
+    }
+}
+
+template <int R, int TT, int RW>
+hipError_t launch_w4_matmul(const W4Args& a, hipStream_t stream) {
+    const uint32_t tiles = R * RW;
+    const dim3 grid((a.row_tiles + tiles - 1u) / tiles, (a.tokens + 16u * TT - 1u) / (16u * TT));
+    const dim3 block(64 * kW4Waves);
+    if (a.group % 128 == 0)
+        hipLaunchKernelGGL((w4_matmul<R, TT, RW, 4>), grid, block, 0, stream, a);
+    else if (a.group % 64 == 0)
+        hipLaunchKernelGGL((w4_matmul<R, TT, RW, 2>), grid, block, 0, stream, a);
+    else
+        hipLaunchKernelGGL((w4_matmul<R, TT, RW, 1>), grid, block, 0, stream, a);
+    return hipGetLastError();
 }
 
 hipError_t launch_w4_narrow(const W4Args& a, bool vec, hipStream_t stream) {
@@ -356,7 +477,7 @@ hipError_t launch_w4_narrow(const W4Args& a, bool vec, hipStream_t stream) {
 
 // Waves per row tile, no more than there are column tiles.  Narrow: enough for eight waves
 // a CU.  Otherwise as many as there are (33 tokens, 2048 x 11008: 14 us with eight, 23 with
-// four; 64 tokens, 12000 x 12000: 59-61 with either).
+// four).
 uint32_t w4_split(uint32_t row_tiles, uint32_t col_tiles, bool narrow, int cus) {
     uint32_t split = 1;
     while (split < kW4Waves && 2u * split <= col_tiles &&
@@ -501,21 +622,37 @@ int attn_w4_matvec(const attn_f16_t* x, attn_f16_t* y, const void* packed,
     const bool vec = aligned16(x) && a.x_stride % 8 == 0 && in_dim % 8 == 0 &&
                      a.x_stride < (1ull << 31) && x_range * 2 < kDead;
     if (a.tokens <= 4) return (int)launch_w4_narrow(a, vec, stream);
-    // Row and token tiles of a wave, by what gives every CU a workgroup (us; tokens x rows x
-    // columns):       1 row tile, 1 token tile   2, 1    4, 2
-    //  16 x 2048 x 2048                     3.9   4.5     8.0
-    //  40 x 500 x 8000                      7.2   9.7    19.3
-    //  33 x 2048 x 11008                   14.4  12.5    23.8
-    //  16 x 12000 x 12000                  25.3  23.0    26.2
-    //  33 x 11008 x 2048                   16.1  13.3    16.3
-    //  64 x 12000 x 12000                  83.4  58.9    50.4
+    // Which kernel, by the workgroups it makes.  P r: own x for every wave, r row tiles; S r t w:
+    // x shared by w waves, r row and t token tiles each (us in a graph; tokens x rows x
+    // columns):              P 1    P 2  S 1 1 2  S 1 1 4  S 1 2 4  S 2 3 4  S 1 4 4
+    //  16 x 4096 x 4096     5.1    6.4    6.5      9.7
+    //  33 x 2048 x 2048     5.6    4.9    4.2      5.4      6.8
+    //  64 x 2048 x 11008   15.4   12.1   15.1     23.5
+    //  16 x 8192 x 8192    12.3   10.2   12.0     18.1
+    //  32 x 8192 x 8192    20.4   15.5   14.1     18.2     24.1
+    //  64 x 11008 x 2048   22.8   18.8   14.9     12.8     13.7     18.6     12.5
+    //  64 x 16384 x 2048   26.6   19.9   14.5     12.3     10.6     12.0     11.7
+    //  48 x 32768 x 4096   58.7   46.2   37.4     33.0     33.0     22.0     28.2
+    //  64 x 128256 x 2048   185    132    102     87.7     67.2     84.0     62.2
     const uint64_t cus = (uint32_t)device_cu_count(device);
     const uint64_t token_tiles = (a.tokens + 15u) / 16u;
-    const uint64_t pairs = (a.tokens + 31u) / 32u;  // of token tiles
-    if (vec && a.tokens > 32 && 32u * pairs - a.tokens < 16u && (a.row_tiles + 3u) / 4u * pairs >= cus)
-        return (int)launch_w4<4, 2>(a, vec, stream);
-    if (a.row_tiles * token_tiles >= cus) return (int)launch_w4<2, 1>(a, vec, stream);
-    return (int)launch_w4<1, 1>(a, vec, stream);
+    if (vec && in_dim > 0) {
+        const uint64_t quads = (a.row_tiles + 3u) / 4u, pairs = (a.row_tiles + 1u) / 2u;
+        // the most token tiles that leave two workgroups a CU
+        for (uint64_t tt = std::min<uint64_t>(4, token_tiles); tt > 0; --tt) {
+            if (quads * ((token_tiles + tt - 1u) / tt) < 2u * cus) continue;
+            if (tt == 4) return (int)launch_w4_matmul<1, 4, 4>(a, stream);
+            if (tt == 3) return (int)launch_w4_matmul<2, 3, 4>(a, stream);
+            if (tt == 2) return (int)launch_w4_matmul<1, 2, 4>(a, stream);
+            return (int)launch_w4_matmul<1, 1, 4>(a, stream);
+        }
+        // more than one a CU, or nearly one and few column tiles (their barriers)
+        const uint64_t groups = pairs * token_tiles;
+        if (groups > cus || (4u * groups >= 3u * cus && a.col_tiles <= 32u))
+            return (int)launch_w4_matmul<1, 1, 2>(a, stream);
+    }
+    if (a.row_tiles * token_tiles > cus) return (int)launch_w4<2>(a, vec, stream);
+    return (int)launch_w4<1>(a, vec, stream);
 }
 
 }  // extern "C"

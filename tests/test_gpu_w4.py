@@ -115,9 +115,12 @@ def test_the_layers_of_a_model(attn, gpu):
 
 
 @pytest.mark.parametrize("group", [32, 64, 128])
-@pytest.mark.parametrize("T,N,K", [(64, 8200, 160), (50, 8208, 200), (100, 6000, 96),
-                                   (64, 8200, 164),   # columns that take element loads
-                                   (16, 4100, 300), (40, 1500, 256)])
+@pytest.mark.parametrize("T,N,K", [
+    (64, 8200, 160), (50, 8208, 200), (100, 6000, 96), (64, 16400, 104), (17, 16390, 72),
+    (64, 32784, 40), (48, 32770, 264), (33, 32768, 48), (16, 32784, 88), (5, 32800, 136),
+    (16, 6150, 1000), (130, 4100, 392), (33, 2060, 640), (64, 2050, 4240),
+    (64, 8200, 164), (20, 32768, 36),   # columns that take element loads
+    (16, 4100, 300), (40, 1500, 256)])
 def test_many_rows(attn, gpu, T, N, K, group):
     """The tiles of more rows and tokens a wave, rows and tokens that end inside them."""
     print(f"[case] T={T} N={N} K={K} group={group}", flush=True)

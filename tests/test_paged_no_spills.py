@@ -9,7 +9,7 @@ import pytest
 CSRC = pathlib.Path(__file__).resolve().parents[1] / "llm-inference_amd" / "csrc"
 
 
-@pytest.mark.parametrize("source,least", [("paged_decode", 24), ("w4_matvec", 14)])
+@pytest.mark.parametrize("source,least", [("paged_decode", 24), ("w4_matvec", 20)])
 def test_kernels_do_not_spill(tmp_path, source, least):
     # the build's own command line for this file
     out = subprocess.run(["make", "-C", str(CSRC), "-n", "-B", f"../lib/obj/{source}.o"],
