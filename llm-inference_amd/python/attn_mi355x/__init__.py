@@ -334,17 +334,23 @@ def _ints(x, what) -> Optional[int]:
     raise AttnError(f"{what} must be a contiguous int32 tensor, got {x.dtype}")
 
 
+# the current device's index, for callers that know CUDA to be initialised
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def _call(fn, what, on, stream, *args):
     """fn(*args, stream) on the device of the tensor `on` (an address: the current one)."""
     if isinstance(on, int):
         rc = fn(*args, _stream(stream))
     else:
-        device = torch.cuda.current_device()
-        if on.get_device() != device:
-            with torch.cuda.device(on.device):
+        index = on.get_device()
+        if index < 0:
+            raise AttnError(f"{what}: tensors must be on a GPU")
+        if index != _current_device():
+            with torch.cuda.device(index):
                 rc = fn(*args, _stream(stream))
         elif stream is None and _raw_stream is not None:
-            rc = fn(*args, _raw_stream(device))
+            rc = fn(*args, _raw_stream(index))
         else:
             rc = fn(*args, _stream(stream))
     if rc != 0:
