@@ -82,6 +82,25 @@ __device__ __forceinline__ u32x4 w4_load(BufRsrc rows, uint32_t byte_off) {
 constexpr uint32_t kW4Waves = 8;
 constexpr uint32_t kDead = 0xfffff000u;  // a buffer offset past every range: nothing is read
 
+// Lane's eight columns of x from column k on, in column tile c, that start at element `at`
+// of xb; zeros past the last.  VEC: rows 16-byte aligned and a multiple of 8 columns, through
+// a range that reads nothing past it.  Otherwise rows at any element: the same 16 bytes as
+// one unaligned load, element by element in the tile that holds the row's end (64 tokens,
+// 2048 x 11009: 15.0 us; 44.1 with elements everywhere, one tile in flight, x not shared).
+template <bool VEC>
+__device__ __forceinline__ f16x8 w4_load_x(BufRsrc rx, const f16* xb, uint64_t at, uint32_t c,
+                                           uint32_t k, uint32_t cols) {
+    if constexpr (VEC) return buf_ld16(rx, k < cols ? 2u * (uint32_t)at : kDead);
+    typedef f16x8 __attribute__((aligned(2))) f16x8_any;
+    if (128u * c + 128u <= cols) return *reinterpret_cast<const f16x8_any*>(xb + at);
+    f16x8 v = {};
+    if (128u * c < cols) {
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) v[e] = k + e < cols ? xb[at + e] : (f16)0.f;
+    }
+    return v;
+}
+
 // index of the scale of column k: k / group.  group_mul is 2^31 over the group in steps of
 // 32 columns, rounded up (0: one group): exact while steps times steps of a group stay
 // below 2^31, as they do up to 2^20 columns.
@@ -127,9 +146,8 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matvec_narrow(W4Args a) {
     if (rt < a.row_tiles && a.col_tiles > 0) {
         const BufRsrc rw =
             make_rsrc(a.w + (uint64_t)rt * a.col_tiles * 256u, a.col_tiles * 1024u);
-        const f16* const xr = a.x + token * a.x_stride;
         const BufRsrc rx = make_rsrc(a.x, (uint32_t)(((a.tokens - 1u) * a.x_stride + a.cols) * 2u));
-        const uint32_t x_at = (uint32_t)(token * a.x_stride) * 2u;
+        const uint64_t x_at = token * a.x_stride;
         const f16* const sc = a.scales + rt * 16u + 4u * gq;
         const uint64_t sc_stride = (uint64_t)a.row_tiles * 16u;
         struct Stage {
@@ -140,12 +158,7 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matvec_narrow(W4Args a) {
         auto load = [&](uint32_t c, Stage& z) {
             z.w = w4_load(rw, c * 1024u + 16u * lane);
             const uint32_t k = 128u * c + 32u * step + 8u * gq;
-            if constexpr (VEC) {
-                z.x = buf_ld16(rx, k < a.cols ? x_at + 2u * k : kDead);
-            } else {
-#pragma unroll
-                for (uint32_t e = 0; e < 8; ++e) z.x[e] = k + e < a.cols ? xr[k + e] : (f16)0.f;
-            }
+            z.x = w4_load_x<VEC>(rx, a.x, x_at + k, c, k, a.cols);
             z.scale = *reinterpret_cast<const f16x4*>(
                 sc + w4_group(a, min(128u * c + 32u * step, a.cols - 1u)) * sc_stride);
         };
@@ -195,7 +208,7 @@ __device__ __forceinline__ f16x4 w4_step_scale(u32x2 mine) {
 // from zero, then scaled and added in fp32, so no product is rounded.
 template <int R, int SPS, bool VEC>
 __global__ __launch_bounds__(64 * kW4Waves) void w4_matvec(W4Args a) {
-    constexpr int kDepth = VEC ? 2 : 1;  // column tiles in flight
+    constexpr int kDepth = 2;  // column tiles in flight
     // a wave's x tile (16 tokens x 128 columns), then the waves' sums
     union Shared {
         f16x8 x[kW4Waves][256];
@@ -247,15 +260,8 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matvec(W4Args a) {
             }
             const uint32_t k = 128u * c + 8u * n;
 #pragma unroll
-            for (uint32_t j = 0; j < 4; ++j) {
-                if constexpr (VEC) {
-                    z.x[j] = buf_ld16(rx, k < a.cols ? 2u * ((uint32_t)x_at[j] + 128u * c) : kDead);
-                } else {
-#pragma unroll
-                    for (uint32_t e = 0; e < 8; ++e)
-                        z.x[j][e] = k + e < a.cols ? xb[x_at[j] + 128u * c + e] : (f16)0.f;
-                }
-            }
+            for (uint32_t j = 0; j < 4; ++j)
+                z.x[j] = w4_load_x<VEC>(rx, xb, x_at[j] + 128u * c, c, k, a.cols);
         };
         auto compute = [&](const Stage& z) {
 #pragma unroll
@@ -327,7 +333,7 @@ hipError_t launch_w4(const W4Args& a, bool vec, hipStream_t stream) {
 // next tile into registers, and one barrier a column tile parts the writes from the reads.
 // Tiles past the last column are zeros through the range checks, so every wave runs the same
 // number of rounds.
-template <int R, int TT, int RW, int SPS>
+template <int R, int TT, int RW, int SPS, bool VEC>
 __global__ __launch_bounds__(64 * kW4Waves) void w4_matmul(W4Args a) {
     constexpr uint32_t kGroups = kW4Waves / RW;
     constexpr int kLoads = 4 * TT / RW;  // of a wave for a tile of x
@@ -355,14 +361,15 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matmul(W4Args a) {
         rw[q] = make_rsrc(a.w + (uint64_t)r * a.col_tiles * 256u, a.col_tiles * 1024u);
         sc[q] = a.scales + r * 16u + 4u * gq;
     }
-    const BufRsrc rx = make_rsrc(a.x + (uint64_t)t0 * a.x_stride,
-                                 (uint32_t)(((live - 1u) * a.x_stride + a.cols) * 2u));
+    const f16* const xb = a.x + (uint64_t)t0 * a.x_stride;
+    const BufRsrc rx = make_rsrc(xb, (uint32_t)(((live - 1u) * a.x_stride + a.cols) * 2u));
     // load i of this wave: rows 4 (rg + RW i) .. + 3 of the token tiles, 256 bytes each
-    uint32_t x_at[kLoads], x_to[kLoads];
+    uint64_t x_at[kLoads];  // elements
+    uint32_t x_to[kLoads];
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
         const uint32_t q = rg + RW * i, r = 4u * (q & 3u) + gq;
-        x_at[i] = 2u * (uint32_t)(min(4u * q + gq, live - 1u) * a.x_stride + 8u * n);
+        x_at[i] = min(4u * q + gq, live - 1u) * a.x_stride + 8u * n;
         x_to[i] = (q >> 2) * 256u + 16u * r + (n ^ r);
     }
     struct Weights {
@@ -373,7 +380,7 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matmul(W4Args a) {
     auto load_x = [&](uint32_t c) {
 #pragma unroll
         for (int i = 0; i < kLoads; ++i)
-            xr[i] = buf_ld16(rx, 128u * c + 8u * n < a.cols ? x_at[i] + 256u * c : kDead);
+            xr[i] = w4_load_x<VEC>(rx, xb, x_at[i] + 128u * c, c, 128u * c + 8u * n, a.cols);
     };
     auto load_w = [&](uint32_t c, Weights& z) {
         const uint64_t at = w4_group(a, min(128u * c + 32u * (n & 3u), a.cols - 1u)) * sc_stride;
@@ -451,18 +458,24 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matmul(W4Args a) {
     }
 }
 
-template <int R, int TT, int RW>
+template <int R, int TT, int RW, bool VEC>
 hipError_t launch_w4_matmul(const W4Args& a, hipStream_t stream) {
     const uint32_t tiles = R * RW;
     const dim3 grid((a.row_tiles + tiles - 1u) / tiles, (a.tokens + 16u * TT - 1u) / (16u * TT));
     const dim3 block(64 * kW4Waves);
     if (a.group % 128 == 0)
-        hipLaunchKernelGGL((w4_matmul<R, TT, RW, 4>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((w4_matmul<R, TT, RW, 4, VEC>), grid, block, 0, stream, a);
     else if (a.group % 64 == 0)
-        hipLaunchKernelGGL((w4_matmul<R, TT, RW, 2>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((w4_matmul<R, TT, RW, 2, VEC>), grid, block, 0, stream, a);
     else
-        hipLaunchKernelGGL((w4_matmul<R, TT, RW, 1>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((w4_matmul<R, TT, RW, 1, VEC>), grid, block, 0, stream, a);
     return hipGetLastError();
+}
+
+template <int R, int TT, int RW>
+hipError_t launch_w4_matmul(const W4Args& a, bool vec, hipStream_t stream) {
+    return vec ? launch_w4_matmul<R, TT, RW, true>(a, stream)
+               : launch_w4_matmul<R, TT, RW, false>(a, stream);
 }
 
 hipError_t launch_w4_narrow(const W4Args& a, bool vec, hipStream_t stream) {
@@ -617,7 +630,7 @@ int attn_w4_matvec(const attn_f16_t* x, attn_f16_t* y, const void* packed,
     const hipError_t e = hipGetDevice(&device);
     if (e != hipSuccess) return (int)e;
     a.split = w4_split(a.row_tiles, a.col_tiles, a.tokens <= 4, device_cu_count(device));
-    // 16-byte reads of x through one 32-bit range per workgroup
+    // reads of x through one 32-bit range per workgroup
     const uint64_t x_range = (std::min<uint64_t>(a.tokens, 64) - 1) * a.x_stride + in_dim;
     const bool vec = aligned16(x) && a.x_stride % 8 == 0 && in_dim % 8 == 0 &&
                      a.x_stride < (1ull << 31) && x_range * 2 < kDead;
@@ -636,20 +649,20 @@ int attn_w4_matvec(const attn_f16_t* x, attn_f16_t* y, const void* packed,
     //  64 x 128256 x 2048   185    132    102     87.7     67.2     84.0     62.2
     const uint64_t cus = (uint32_t)device_cu_count(device);
     const uint64_t token_tiles = (a.tokens + 15u) / 16u;
-    if (vec && in_dim > 0) {
+    if (in_dim > 0) {
         const uint64_t quads = (a.row_tiles + 3u) / 4u, pairs = (a.row_tiles + 1u) / 2u;
         // the most token tiles that leave two workgroups a CU
         for (uint64_t tt = std::min<uint64_t>(4, token_tiles); tt > 0; --tt) {
             if (quads * ((token_tiles + tt - 1u) / tt) < 2u * cus) continue;
-            if (tt == 4) return (int)launch_w4_matmul<1, 4, 4>(a, stream);
-            if (tt == 3) return (int)launch_w4_matmul<2, 3, 4>(a, stream);
-            if (tt == 2) return (int)launch_w4_matmul<1, 2, 4>(a, stream);
-            return (int)launch_w4_matmul<1, 1, 4>(a, stream);
+            if (tt == 4) return (int)launch_w4_matmul<1, 4, 4>(a, vec, stream);
+            if (tt == 3) return (int)launch_w4_matmul<2, 3, 4>(a, vec, stream);
+            if (tt == 2) return (int)launch_w4_matmul<1, 2, 4>(a, vec, stream);
+            return (int)launch_w4_matmul<1, 1, 4>(a, vec, stream);
         }
         // more than one a CU, or nearly one and few column tiles (their barriers)
         const uint64_t groups = pairs * token_tiles;
         if (groups > cus || (4u * groups >= 3u * cus && a.col_tiles <= 32u))
-            return (int)launch_w4_matmul<1, 1, 2>(a, stream);
+            return (int)launch_w4_matmul<1, 1, 2>(a, vec, stream);
     }
     if (a.row_tiles * token_tiles > cus) return (int)launch_w4<2>(a, vec, stream);
     return (int)launch_w4<1>(a, vec, stream);

@@ -127,6 +127,17 @@ def test_many_rows(attn, gpu, T, N, K, group):
     product(attn, gpu, T, N, K, group, T, residual="apart")
 
 
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("T,N,K", [
+    (1, 40, 1027), (4, 100, 2050), (12, 60, 1281), (16, 4100, 447), (16, 6150, 1001), (33, 2060, 641),
+    (64, 8200, 161), (40, 16400, 199), (100, 6000, 97), (48, 32770, 261), (5, 32800, 135),
+    (64, 2050, 4241), (65, 16400, 5), (20, 300, 127), (20, 300, 129)])
+def test_odd_columns(attn, gpu, T, N, K, group):
+    """Rows of x at every element: no 16-byte boundary, the tile with the row's end."""
+    print(f"[case] T={T} N={N} K={K} group={group}", flush=True)
+    product(attn, gpu, T, N, K, group, T, x_off=T % 3)
+
+
 def test_infinity_in_one_token_stays_there(attn, gpu):
     N, K = 40, 200
     codes, scales = weights(N, K, 32, 1)
