@@ -198,7 +198,7 @@ __device__ __forceinline__ f16x4 w4_step_scale(u32x2 mine) {
     u32x2 v;
 #pragma unroll
     for (int i = 0; i < 2; ++i)  // quad_perm [S, S, S, S]
-        v[i] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)mine[i], S * 0x55, 0xF, 0xF, false);
+        v[i] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)mine[i], S * 0x55, 0xF, 0xF, true);
     return __builtin_bit_cast(f16x4, v);
 }
 
