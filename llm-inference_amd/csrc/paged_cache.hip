@@ -268,7 +268,7 @@ __global__ __launch_bounds__(kPlanThreads) void pages_grow_plan(GrowArgs a) {
     uint32_t found = 0;
     if (s_short == 0 && need_all > 0) {
         int4 r = load_refs(a.refs, 4u * tid, a.num_pages);
-        uint32_t which = 0;
+        uint32_t which = 0, looked = 0;
         for (uint32_t base = 0; base < a.num_pages && (int64_t)found < need_all; base += kPlanTile) {
             const uint32_t p = base + 4u * tid;
             const int4 next = load_refs(a.refs, p + kPlanTile, a.num_pages);  // the next round's
@@ -284,6 +284,30 @@ __global__ __launch_bounds__(kPlanThreads) void pages_grow_plan(GrowArgs a) {
             found += total;
             r = next;
             which ^= 1u;
+            // After a round without a free page four rounds' pages at a time are passed over
+            // while none of them is free (170000 pages, all in use but the last ones: 20.0 us
+            // against 30.4 round by round), not again before the four that hold one are done.
+            if (total == 0 && base >= looked) {
+                const uint32_t near = base + kPlanTile;
+                uint32_t far = near;
+                while (far + 4u * kPlanTile <= a.num_pages) {
+                    int4 q[4];
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i)
+                        q[i] = load_refs(a.refs, far + i * kPlanTile + 4u * tid, a.num_pages);
+                    bool any = false;
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i)
+                        any |= q[i].x == 0 || q[i].y == 0 || q[i].z == 0 || q[i].w == 0;
+                    if (__syncthreads_or(any)) break;
+                    far += 4u * kPlanTile;
+                }
+                looked = far + 4u * kPlanTile;
+                if (far != near) {
+                    base = far - kPlanTile;
+                    r = load_refs(a.refs, far + 4u * tid, a.num_pages);
+                }
+            }
         }
     }
     __syncthreads();

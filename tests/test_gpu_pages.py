@@ -98,6 +98,43 @@ def test_short_pool_changes_nothing(attn, gpu):
     assert x.grow([-2**31, 0, 0]) == (0, 0)
 
 
+@pytest.mark.parametrize("pages", [20479, 20480, 20481, 40000, 70001, 174080])
+@pytest.mark.parametrize("where", ["last", "few", "one a round", "far apart", "none"])
+def test_free_pages_far_up_a_large_pool(attn, gpu, pages, where):
+    """The lowest free pages lie behind thousands that are in use."""
+    print(f"[case] {pages} pages, {where}", flush=True)
+    rng = np.random.default_rng(pages)
+    free = {"last": [pages - 1], "none": [], "few": sorted(rng.choice(pages, 5, replace=False)),
+            "one a round": list(range(4095, pages, 4096)),
+            "far apart": [p for p in (3, 4095, 4096, 20479, 20480, 36863, 36864, 53247, 69999,
+                                      150000, pages - 2) if p < pages]}[where]
+    free = sorted({int(p) for p in free})
+    seqs, columns = 7, 16
+    cache = attn.PagedKVCache(1, pages, 1, 1, 8, seqs, columns, gpu)
+    pool = cache.pool.view(torch.int16).clone()
+    for need in sorted({min(len(free), 1), min(len(free), 4), min(len(free), 60), len(free) + 1}):
+        refs = torch.ones(pages, dtype=torch.int32)
+        refs[free] = 0
+        cache.ref_counts.copy_(refs)
+        cache.seq_lens.zero_()
+        cache.page_table.fill_(-1)
+        grow = [min(columns, max(0, need - columns * b)) for b in range(seqs)]
+        cache.grow(torch.tensor(grow, dtype=torch.int32, device=gpu))
+        torch.cuda.synchronize()
+        if need > len(free):
+            assert cache.status.tolist() == [1, 0]
+            assert cache.seq_lens.tolist() == [0] * seqs
+        else:
+            assert cache.status.tolist() == [0, 0]
+            assert cache.seq_lens.tolist() == grow
+            table = cache.page_table.cpu().reshape(seqs, columns)
+            taken = [int(table[b, j]) for b in range(seqs) for j in range(grow[b])]
+            assert taken == free[:need]
+            refs[taken] = 1
+        assert torch.equal(cache.ref_counts.cpu(), refs)
+    assert torch.equal(cache.pool.view(torch.int16), pool)
+
+
 def test_forks_copy_their_last_page_when_they_grow(attn, gpu):
     x = Both(attn, gpu, 2, 30, 4, 1, 8, 6, 6, 2)
     x.grow([6, 8, 0, 0, 0, 0])                  # row 0 ends inside a page, row 1 at its end
