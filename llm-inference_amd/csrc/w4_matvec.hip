@@ -14,12 +14,13 @@
 // zero in rows past the matrix.
 //
 // Bound by the weights' bytes for a few tokens and many rows (one token, 128256 x 2048: 135.7
-// MB in 26.7 us, 5.1 TB/s), by latency for few rows (2048 x 2048: 4.0 us).  For a batch
-// the workgroups' reads of x bound it: each reads its tokens' whole rows from the L2, at
-// about 9 ns a KiB and CU (33 tokens, 2048 x 11008, groups of 32: 14.4 us, of which the
-// weights' 11.3 MB would take 2.7).  Many rows share those reads between the waves of a
-// workgroup; for few rows, sharing the columns between workgroups would divide them, but
-// takes a workspace and a second kernel for the sums.
+// MB in 26.7 us, 5.1 TB/s), by latency for few rows (2048 x 2048: 3.2 us).  For a batch
+// the load pipe and the unpacking bound it (33 tokens, 2048 x 11008, groups of 32: 12.6 us,
+// of which the weights' 11.3 MB would take 2.7): each workgroup reads its tokens' whole rows
+// of x, about 9 ns a KiB and CU wherever they lie, and the vector instructions take half
+// the time.  Many rows share those reads between the waves of a workgroup; for few rows,
+// sharing the columns between workgroups would divide them, but takes a workspace and a
+// second kernel for the sums.
 #include "attn_internal.hpp"
 #include "../../include/attn_mi355x.h"
 
@@ -127,7 +128,35 @@ __device__ __forceinline__ void w4_store(const W4Args& a, const float (*s_part)[
     }
 }
 
-// Up to four tokens.  Column n of the MFMAs' result stands for token n / 4 and step n % 4
+// A wave's column tiles first, first + step, .. below end, with D of them in flight.  Nothing
+// past the end is loaded: a load that reads nothing holds the load pipe as long as any (one
+// token, 2048 x 2048: 3.2 us against 3.8; 16 tokens, 4096 x 4096: 5.3 against 5.5).
+template <int D, class Stage, class Load, class Compute>
+__device__ __forceinline__ void w4_columns(uint32_t first, uint32_t step, uint32_t end,
+                                           Stage (&st)[D], const Load& load,
+                                           const Compute& compute) {
+    uint32_t c = first;
+#pragma unroll
+    for (int i = 0; i < D; ++i)
+        if (c + i * step < end) load(c + i * step, st[i]);
+    for (; c + (2 * D - 1) * step < end; c += D * step) {
+#pragma unroll
+        for (int i = 0; i < D; ++i) {
+            __builtin_amdgcn_sched_barrier(0);
+            compute(st[i]);
+            load(c + (i + D) * step, st[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * D - 1; ++i) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (c + i * step >= end) break;
+        compute(st[i % D]);
+        if (i < D - 1 && c + (i + D) * step < end) load(c + (i + D) * step, st[i % D]);
+    }
+}
+
+// Up to four tokens.  Column n of the MFMAs' result stands for token n % 4 and step n / 4
 // of a column tile: lane (gq, n) loads x for that step only (one load per column tile
 // instead of four), the operand of step s is zero in the other steps' columns, and each
 // lane scales its column's sum by its own step's scales, whatever the group size.
@@ -137,11 +166,11 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matvec_narrow(W4Args a) {
     __shared__ float s_part[kW4Waves][4][17];
     const uint32_t lane = threadIdx.x & 63u;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t n = lane & 15u, gq = lane >> 4, step = n & 3u;
+    const uint32_t n = lane & 15u, gq = lane >> 4, step = n >> 2;
     const W4Consts consts;
     const uint32_t rt = (blockIdx.x * kW4Waves + wave) / a.split;
     const uint32_t first = wave & (a.split - 1u);
-    const uint32_t token = min(n >> 2, a.tokens - 1u);
+    const uint32_t token = min(n & 3u, a.tokens - 1u);
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     if (rt < a.row_tiles && a.col_tiles > 0) {
         const BufRsrc rw =
@@ -162,43 +191,34 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matvec_narrow(W4Args a) {
             z.scale = *reinterpret_cast<const f16x4*>(
                 sc + w4_group(a, min(128u * c + 32u * step, a.cols - 1u)) * sc_stride);
         };
+        auto compute = [&](const Stage& z) {
+            f32x4 part = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < kDepth; ++i) load(first + i * a.split, st[i]);
-        for (uint32_t c = first; c < a.col_tiles; c += kDepth * a.split) {
+            for (uint32_t s = 0; s < 4; ++s)
+                part = mfma16(w4_values(z.w[s], consts), step == s ? z.x : f16x8{}, part);
 #pragma unroll
-            for (int i = 0; i < kDepth; ++i) {
-                __builtin_amdgcn_sched_barrier(0);
-                if (c + i * a.split < a.col_tiles) {
-                    f32x4 part = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (uint32_t s = 0; s < 4; ++s)
-                        part = mfma16(w4_values(st[i].w[s], consts), step == s ? st[i].x : f16x8{}, part);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        acc[r] = __builtin_fmaf((float)st[i].scale[r], part[r], acc[r]);
-                }
-                load(c + (i + kDepth) * a.split, st[i]);
-            }
-        }
+            for (int r = 0; r < 4; ++r) acc[r] = __builtin_fmaf((float)z.scale[r], part[r], acc[r]);
+        };
+        w4_columns<kDepth>(first, a.split, a.col_tiles, st, load, compute);
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {  // the four steps of a token
         float v = acc[r];
-        v += dpp_f<kDppXor1>(v);
-        v += dpp_f<kDppXor2>(v);
-        if (step == 0) s_part[wave][n >> 2][4u * gq + r] = v;
+        v += dpp_f<kDppRor4>(v);
+        v += dpp_f<kDppRor8>(v);
+        if (step == 0) s_part[wave][n][4u * gq + r] = v;
     }
     __syncthreads();
     w4_store<4, 1>(a, s_part, 0, a.tokens);
 }
 
-// the scales that lane step % 4 of each four lanes loaded, in all four
-template <int S>
-__device__ __forceinline__ f16x4 w4_step_scale(u32x2 mine) {
+// the scales that lane L of a row of 16 lanes loaded, in all of them
+template <int L>
+__device__ __forceinline__ f16x4 w4_lane_scale(u32x2 mine) {
     u32x2 v;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)  // quad_perm [S, S, S, S]
-        v[i] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)mine[i], S * 0x55, 0xF, 0xF, true);
+    for (int i = 0; i < 2; ++i)  // row_newbcast L
+        v[i] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)mine[i], 0x150 + L, 0xF, 0xF, true);
     return __builtin_bit_cast(f16x4, v);
 }
 
@@ -228,14 +248,15 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matvec(W4Args a) {
     for (int q = 0; q < R; ++q) acc[q] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (rt < a.row_tiles && a.col_tiles > 0) {
         BufRsrc rw[R];
-        const f16* sc[R];
-        const uint64_t sc_stride = (uint64_t)a.row_tiles * 16u;
 #pragma unroll
-        for (int q = 0; q < R; ++q) {  // row tiles past the last one repeat it and are not stored
-            const uint32_t r = min(rt + q, a.row_tiles - 1u);
-            rw[q] = make_rsrc(a.w + (uint64_t)r * a.col_tiles * 256u, a.col_tiles * 1024u);
-            sc[q] = a.scales + r * 16u + 4u * gq;
-        }
+        for (int q = 0; q < R; ++q)  // row tiles past the last one repeat it and are not stored
+            rw[q] = make_rsrc(a.w + (uint64_t)min(rt + q, a.row_tiles - 1u) * a.col_tiles * 256u,
+                              a.col_tiles * 1024u);
+        // Lane n takes the scales of step n / 4 and row tile n % R: one load, whose lanes on
+        // the same line are neighbours (33 tokens, 2048 x 11008, groups of 32: 13.1 us
+        // against 14.3 with step n % 4 and a load per row tile).
+        const f16* const sc = a.scales + min(rt + n % R, a.row_tiles - 1u) * 16u + 4u * gq;
+        const uint64_t sc_stride = (uint64_t)a.row_tiles * 16u;
         const f16* const xb = a.x + (uint64_t)t0 * a.x_stride;
         const BufRsrc rx = make_rsrc(xb, (uint32_t)(((live - 1u) * a.x_stride + a.cols) * 2u));
         // x is read in whole lines, four rows of 256 bytes an instruction (16 rows of 64
@@ -249,15 +270,13 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matvec(W4Args a) {
         struct Stage {
             u32x4 w[R];
             f16x8 x[4];
-            u32x2 scale[R];  // of step n % 4, rows 4 gq ..
+            u32x2 scale;  // rows 4 gq ..
         } st[kDepth];
         auto load = [&](uint32_t c, Stage& z) {
-            const uint64_t at = w4_group(a, min(128u * c + 32u * (n & 3u), a.cols - 1u)) * sc_stride;
 #pragma unroll
-            for (int q = 0; q < R; ++q) {
-                z.w[q] = w4_load(rw[q], c * 1024u + 16u * lane);
-                z.scale[q] = *reinterpret_cast<const u32x2*>(sc[q] + at);
-            }
+            for (int q = 0; q < R; ++q) z.w[q] = w4_load(rw[q], c * 1024u + 16u * lane);
+            z.scale = *reinterpret_cast<const u32x2*>(
+                sc + w4_group(a, min(128u * c + 32u * (n >> 2), a.cols - 1u)) * sc_stride);
             const uint32_t k = 128u * c + 8u * n;
 #pragma unroll
             for (uint32_t j = 0; j < 4; ++j)
@@ -275,7 +294,8 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matvec(W4Args a) {
 #pragma unroll
                 for (int q = 0; q < R; ++q) {
                     const f16x8 wv = w4_values(z.w[q][s], consts);
-                    const f16x4 scale = w4_step_scale<s>(z.scale[q]);
+                    const f16x4 scale =
+                    q == 0 ? w4_lane_scale<4 * s>(z.scale) : w4_lane_scale<4 * s + 1>(z.scale);
                     if (s % SPS == 0) part[q] = f32x4{0.f, 0.f, 0.f, 0.f};
                     part[q] = mfma16(wv, xv, part[q]);
                     if (s % SPS == SPS - 1)
@@ -289,16 +309,7 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matvec(W4Args a) {
             step.template operator()<2>();
             step.template operator()<3>();
         };
-#pragma unroll
-        for (int i = 0; i < kDepth; ++i) load(first + i * a.split, st[i]);
-        for (uint32_t c = first; c < a.col_tiles; c += kDepth * a.split) {
-#pragma unroll
-            for (int i = 0; i < kDepth; ++i) {
-                __builtin_amdgcn_sched_barrier(0);
-                if (c + i * a.split < a.col_tiles) compute(st[i]);
-                load(c + (i + kDepth) * a.split, st[i]);
-            }
-        }
+        w4_columns<kDepth>(first, a.split, a.col_tiles, st, load, compute);
     }
     __syncthreads();  // every wave has read its x tiles
 #pragma unroll
@@ -353,14 +364,13 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matmul(W4Args a) {
     const uint32_t live = min(a.tokens - t0, 16u * (uint32_t)TT);
     const W4Consts consts;
     BufRsrc rw[R];
-    const f16* sc[R];
-    const uint64_t sc_stride = (uint64_t)a.row_tiles * 16u;
 #pragma unroll
-    for (int q = 0; q < R; ++q) {  // row tiles past the last one repeat it and are not stored
-        const uint32_t r = min(rt + q, a.row_tiles - 1u);
-        rw[q] = make_rsrc(a.w + (uint64_t)r * a.col_tiles * 256u, a.col_tiles * 1024u);
-        sc[q] = a.scales + r * 16u + 4u * gq;
-    }
+    for (int q = 0; q < R; ++q)  // row tiles past the last one repeat it and are not stored
+        rw[q] = make_rsrc(a.w + (uint64_t)min(rt + q, a.row_tiles - 1u) * a.col_tiles * 256u,
+                          a.col_tiles * 1024u);
+    // lane n takes the scales of step n / 4 and row tile n % R
+    const f16* const sc = a.scales + min(rt + n % R, a.row_tiles - 1u) * 16u + 4u * gq;
+    const uint64_t sc_stride = (uint64_t)a.row_tiles * 16u;
     const f16* const xb = a.x + (uint64_t)t0 * a.x_stride;
     const BufRsrc rx = make_rsrc(xb, (uint32_t)(((live - 1u) * a.x_stride + a.cols) * 2u));
     // load i of this wave: rows 4 (rg + RW i) .. + 3 of the token tiles, 256 bytes each
@@ -374,7 +384,7 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matmul(W4Args a) {
     }
     struct Weights {
         u32x4 w[R];
-        u32x2 scale[R];  // of step n % 4, rows 4 gq ..
+        u32x2 scale;  // rows 4 gq ..
     };
     f16x8 xr[kLoads];
     auto load_x = [&](uint32_t c) {
@@ -383,12 +393,10 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matmul(W4Args a) {
             xr[i] = w4_load_x<VEC>(rx, xb, x_at[i] + 128u * c, c, 128u * c + 8u * n, a.cols);
     };
     auto load_w = [&](uint32_t c, Weights& z) {
-        const uint64_t at = w4_group(a, min(128u * c + 32u * (n & 3u), a.cols - 1u)) * sc_stride;
 #pragma unroll
-        for (int q = 0; q < R; ++q) {
-            z.w[q] = w4_load(rw[q], c * 1024u + 16u * lane);
-            z.scale[q] = *reinterpret_cast<const u32x2*>(sc[q] + at);
-        }
+        for (int q = 0; q < R; ++q) z.w[q] = w4_load(rw[q], c * 1024u + 16u * lane);
+        z.scale = *reinterpret_cast<const u32x2*>(
+            sc + w4_group(a, min(128u * c + 32u * (n >> 2), a.cols - 1u)) * sc_stride);
     };
     f32x4 acc[R][TT];
 #pragma unroll
@@ -404,7 +412,8 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matmul(W4Args a) {
 #pragma unroll
             for (int q = 0; q < R; ++q) {
                 const f16x8 wv = w4_values(z.w[q][s], consts);
-                const f16x4 scale = w4_step_scale<s>(z.scale[q]);
+                const f16x4 scale =
+                    q == 0 ? w4_lane_scale<4 * s>(z.scale) : w4_lane_scale<4 * s + 1>(z.scale);
 #pragma unroll
                 for (int tt = 0; tt < TT; ++tt) {
                     if (s % SPS == 0) part[q][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
