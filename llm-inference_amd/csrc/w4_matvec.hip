@@ -338,18 +338,18 @@ hipError_t launch_w4(const W4Args& a, bool vec, hipStream_t stream) {
     return launch_w4<R, 1>(a, vec, stream);
 }
 
-// Many rows and tokens: RW of the eight waves take row tiles of their own (R each) and share
-// x, so that a workgroup reads x once for 16 R RW rows; the 8 / RW groups of waves split the
-// columns.  x goes through two LDS tiles in turn: each wave of a group loads its part of the
+// Many rows and tokens: RW of the eight waves take row tiles of their own and share x, so
+// that a workgroup reads x once for 16 RW rows and unpacks codes once for 16 TT tokens; the
+// 8 / RW groups of waves split the columns.  x goes through two LDS tiles in turn: each wave of a group loads its part of the
 // next tile into registers, and one barrier a column tile parts the writes from the reads.
 // Tiles past the last column are zeros through the range checks, so every wave runs the same
 // number of rounds.
-template <int R, int TT, int RW, int SPS, bool VEC>
+template <int TT, int RW, int SPS, bool VEC>
 __global__ __launch_bounds__(64 * kW4Waves) void w4_matmul(W4Args a) {
     constexpr uint32_t kGroups = kW4Waves / RW;
     constexpr int kLoads = 4 * TT / RW;  // of a wave for a tile of x
     static_assert(kLoads * RW == 4 * TT);
-    constexpr uint32_t kRows = 16 * R * RW;
+    constexpr uint32_t kRows = 16 * RW;
     union Shared {
         f16x8 x[2][kGroups][TT][256];
         float part[kGroups][16 * TT][kRows + 1];
@@ -359,17 +359,14 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matmul(W4Args a) {
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t n = lane & 15u, gq = lane >> 4;
     const uint32_t kg = wave / RW, rg = wave % RW;
-    const uint32_t rt = (blockIdx.x * RW + rg) * R;
+    // a row tile past the last one repeats it and is not stored
+    const uint32_t rt = min(blockIdx.x * RW + rg, a.row_tiles - 1u);
     const uint32_t t0 = blockIdx.y * 16u * TT;
     const uint32_t live = min(a.tokens - t0, 16u * (uint32_t)TT);
     const W4Consts consts;
-    BufRsrc rw[R];
-#pragma unroll
-    for (int q = 0; q < R; ++q)  // row tiles past the last one repeat it and are not stored
-        rw[q] = make_rsrc(a.w + (uint64_t)min(rt + q, a.row_tiles - 1u) * a.col_tiles * 256u,
-                          a.col_tiles * 1024u);
-    // lane n takes the scales of step n / 4 and row tile n % R
-    const f16* const sc = a.scales + min(rt + n % R, a.row_tiles - 1u) * 16u + 4u * gq;
+    const BufRsrc rw = make_rsrc(a.w + (uint64_t)rt * a.col_tiles * 256u, a.col_tiles * 1024u);
+    // lane n takes the scales of step n / 4
+    const f16* const sc = a.scales + rt * 16u + 4u * gq;
     const uint64_t sc_stride = (uint64_t)a.row_tiles * 16u;
     const f16* const xb = a.x + (uint64_t)t0 * a.x_stride;
     const BufRsrc rx = make_rsrc(xb, (uint32_t)(((live - 1u) * a.x_stride + a.cols) * 2u));
@@ -383,7 +380,7 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matmul(W4Args a) {
         x_to[i] = (q >> 2) * 256u + 16u * r + (n ^ r);
     }
     struct Weights {
-        u32x4 w[R];
+        u32x4 w;
         u32x2 scale;  // rows 4 gq ..
     };
     f16x8 xr[kLoads];
@@ -393,43 +390,52 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matmul(W4Args a) {
             xr[i] = w4_load_x<VEC>(rx, xb, x_at[i] + 128u * c, c, 128u * c + 8u * n, a.cols);
     };
     auto load_w = [&](uint32_t c, Weights& z) {
-#pragma unroll
-        for (int q = 0; q < R; ++q) z.w[q] = w4_load(rw[q], c * 1024u + 16u * lane);
+        z.w = w4_load(rw, c * 1024u + 16u * lane);
         z.scale = *reinterpret_cast<const u32x2*>(
             sc + w4_group(a, min(128u * c + 32u * (n >> 2), a.cols - 1u)) * sc_stride);
     };
-    f32x4 acc[R][TT];
+    f32x4 acc[TT];
 #pragma unroll
-    for (int q = 0; q < R; ++q)
-#pragma unroll
-        for (int tt = 0; tt < TT; ++tt) acc[q][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int tt = 0; tt < TT; ++tt) acc[tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // Groups of 32, three token tiles and more: a step's sums are scaled after the next
+    // step's products, which hide the MFMAs' latency (48 tokens, 16384 x 4096: 18.3 us
+    // against 22.9; with wider groups the compiler's order is the better one, 15.4 against
+    // 17.2 with groups of 64).
+    constexpr bool kLate = SPS == 1 && TT > 2;
     auto compute = [&](const f16x8 (*x)[256], const Weights& z) {
-        f32x4 part[R][TT];
+        f32x4 part[kLate ? 2 : 1][TT];
+        auto add = [&]<int g>() {
+            const f16x4 scale = w4_lane_scale<4 * SPS * g>(z.scale);
+#pragma unroll
+            for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    acc[tt][r] =
+                        __builtin_fmaf((float)scale[r], part[kLate ? g & 1 : 0][tt][r], acc[tt][r]);
+        };
         auto step = [&]<int s>() {
+            constexpr int g = s / SPS, p = kLate ? g & 1 : 0;
             f16x8 xv[TT];
 #pragma unroll
             for (int tt = 0; tt < TT; ++tt) xv[tt] = x[tt][16u * n + ((4u * s + gq) ^ n)];
+            const f16x8 wv = w4_values(z.w[s], consts);
 #pragma unroll
-            for (int q = 0; q < R; ++q) {
-                const f16x8 wv = w4_values(z.w[q][s], consts);
-                const f16x4 scale =
-                    q == 0 ? w4_lane_scale<4 * s>(z.scale) : w4_lane_scale<4 * s + 1>(z.scale);
-#pragma unroll
-                for (int tt = 0; tt < TT; ++tt) {
-                    if (s % SPS == 0) part[q][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
-                    part[q][tt] = mfma16(wv, xv[tt], part[q][tt]);
-                    if (s % SPS == SPS - 1)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            acc[q][tt][r] =
-                                __builtin_fmaf((float)scale[r], part[q][tt][r], acc[q][tt][r]);
-                }
+            for (int tt = 0; tt < TT; ++tt) {
+                if (s % SPS == 0) part[p][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+                part[p][tt] = mfma16(wv, xv[tt], part[p][tt]);
             }
+            if constexpr (kLate && s > 0) {
+                __builtin_amdgcn_sched_barrier(0);
+                add.template operator()<g - 1>();
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if constexpr (!kLate && s % SPS == SPS - 1) add.template operator()<g>();
         };
         step.template operator()<0>();
         step.template operator()<1>();
         step.template operator()<2>();
         step.template operator()<3>();
+        if constexpr (kLate) add.template operator()<3>();
     };
     Weights wa, wb;
     load_w(kg, wa);
@@ -448,12 +454,10 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matmul(W4Args a) {
     }
     __syncthreads();  // x is read
 #pragma unroll
-    for (int q = 0; q < R; ++q)
+    for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
-        for (int tt = 0; tt < TT; ++tt)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                s_mem.part[kg][16 * tt + n][16u * (R * rg + q) + 4u * gq + r] = acc[q][tt][r];
+        for (int r = 0; r < 4; ++r)
+            s_mem.part[kg][16 * tt + n][16u * rg + 4u * gq + r] = acc[tt][r];
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < live * kRows; i += 64u * kW4Waves) {
         const uint32_t t = i / kRows, r = i % kRows, row = blockIdx.x * kRows + r;
@@ -467,24 +471,23 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matmul(W4Args a) {
     }
 }
 
-template <int R, int TT, int RW, bool VEC>
+template <int TT, int RW, bool VEC>
 hipError_t launch_w4_matmul(const W4Args& a, hipStream_t stream) {
-    const uint32_t tiles = R * RW;
-    const dim3 grid((a.row_tiles + tiles - 1u) / tiles, (a.tokens + 16u * TT - 1u) / (16u * TT));
+    const dim3 grid((a.row_tiles + RW - 1u) / RW, (a.tokens + 16u * TT - 1u) / (16u * TT));
     const dim3 block(64 * kW4Waves);
     if (a.group % 128 == 0)
-        hipLaunchKernelGGL((w4_matmul<R, TT, RW, 4, VEC>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((w4_matmul<TT, RW, 4, VEC>), grid, block, 0, stream, a);
     else if (a.group % 64 == 0)
-        hipLaunchKernelGGL((w4_matmul<R, TT, RW, 2, VEC>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((w4_matmul<TT, RW, 2, VEC>), grid, block, 0, stream, a);
     else
-        hipLaunchKernelGGL((w4_matmul<R, TT, RW, 1, VEC>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((w4_matmul<TT, RW, 1, VEC>), grid, block, 0, stream, a);
     return hipGetLastError();
 }
 
-template <int R, int TT, int RW>
+template <int TT, int RW>
 hipError_t launch_w4_matmul(const W4Args& a, bool vec, hipStream_t stream) {
-    return vec ? launch_w4_matmul<R, TT, RW, true>(a, stream)
-               : launch_w4_matmul<R, TT, RW, false>(a, stream);
+    return vec ? launch_w4_matmul<TT, RW, true>(a, stream)
+               : launch_w4_matmul<TT, RW, false>(a, stream);
 }
 
 hipError_t launch_w4_narrow(const W4Args& a, bool vec, hipStream_t stream) {
@@ -644,34 +647,47 @@ int attn_w4_matvec(const attn_f16_t* x, attn_f16_t* y, const void* packed,
     const bool vec = aligned16(x) && a.x_stride % 8 == 0 && in_dim % 8 == 0 &&
                      a.x_stride < (1ull << 31) && x_range * 2 < kDead;
     if (a.tokens <= 4) return (int)launch_w4_narrow(a, vec, stream);
-    // Which kernel, by the workgroups it makes.  P r: own x for every wave, r row tiles; S r t w:
-    // x shared by w waves, r row and t token tiles each (us in a graph; tokens x rows x
-    // columns):              P 1    P 2  S 1 1 2  S 1 1 4  S 1 2 4  S 2 3 4  S 1 4 4
-    //  16 x 4096 x 4096     5.1    6.4    6.5      9.7
-    //  33 x 2048 x 2048     5.6    4.9    4.2      5.4      6.8
-    //  64 x 2048 x 11008   15.4   12.1   15.1     23.5
-    //  16 x 8192 x 8192    12.3   10.2   12.0     18.1
-    //  32 x 8192 x 8192    20.4   15.5   14.1     18.2     24.1
-    //  64 x 11008 x 2048   22.8   18.8   14.9     12.8     13.7     18.6     12.5
-    //  64 x 16384 x 2048   26.6   19.9   14.5     12.3     10.6     12.0     11.7
-    //  48 x 32768 x 4096   58.7   46.2   37.4     33.0     33.0     22.0     28.2
-    //  64 x 128256 x 2048   185    132    102     87.7     67.2     84.0     62.2
+    // Which kernel, by the workgroups it makes.  P r: own x for every wave, r row tiles; S t w:
+    // x shared by w waves of a row tile each, t token tiles (us in a graph, groups of 64;
+    // tokens x rows x columns, CUs 256):
+    //                       P 1    P 2   S 1 2   S 1 4   S 2 4   S 3 4   S 4 4
+    //  16 x 4096 x 4096     5.4    6.1    6.6     9.8    10.9    13.6    16.6
+    //  16 x 8192 x 8192    12.4   10.7   12.3    18.3    20.2    24.7    30.4
+    //  16 x 11008 x 2048    7.0    6.3    5.7     6.7     7.3     8.6    10.0
+    //  16 x 128256 x 2048  49.8   38.0   33.6    29.4    37.3    46.7    55.5
+    //  33 x 2048 x 2048     4.7    4.3    4.1     5.2     6.5     8.2     9.6
+    //  64 x 2048 x 11008   14.8   12.0   15.0    23.4    26.3    33.6    40.6
+    //  32 x 8192 x 8192    20.8   15.5   14.4    18.3    20.1    24.8    30.7
+    //  32 x 11008 x 2048           8.1    7.2     8.4     7.4     8.7    10.1
+    //  32 x 24000 x 2048   18.1   14.8   12.4    11.7    10.2    12.5    14.8
+    //  48 x 8192 x 4096    16.3   13.2   11.5    12.7    11.9    14.4    16.8
+    //  48 x 11008 x 2048          11.3    9.9    10.2     9.8     8.9    10.1
+    //  48 x 16384 x 4096          23.4   20.2    18.4    17.2    15.3    18.1
+    //  64 x 8192 x 8192    36.4   26.5   24.8    22.6    20.5    26.3    30.2
+    //  64 x 12000 x 12000  82.9   57.6   56.0    50.0    43.8    56.1    47.6
+    //  64 x 30000 x 2048          32.2   26.3    26.0    19.4    24.2    16.9
+    //  64 x 128256 x 2048   160    122    106    91.9    66.1    90.5    63.2
+    //  96 x 6000 x 4096    22.8   18.9   16.9    17.6    16.6    14.7    17.4
     const uint64_t cus = (uint32_t)device_cu_count(device);
     const uint64_t token_tiles = (a.tokens + 15u) / 16u;
     if (in_dim > 0) {
         const uint64_t quads = (a.row_tiles + 3u) / 4u, pairs = (a.row_tiles + 1u) / 2u;
-        // the most token tiles that leave two workgroups a CU
+        // the most token tiles that fit the tokens (a fifth more at most) and leave enough
+        // workgroups, in twelfths of the CUs
+        const uint64_t enough[5] = {0, 48, 9, 8, 21};
         for (uint64_t tt = std::min<uint64_t>(4, token_tiles); tt > 0; --tt) {
-            if (quads * ((token_tiles + tt - 1u) / tt) < 2u * cus) continue;
-            if (tt == 4) return (int)launch_w4_matmul<1, 4, 4>(a, vec, stream);
-            if (tt == 3) return (int)launch_w4_matmul<2, 3, 4>(a, vec, stream);
-            if (tt == 2) return (int)launch_w4_matmul<1, 2, 4>(a, vec, stream);
-            return (int)launch_w4_matmul<1, 1, 4>(a, vec, stream);
+            const uint64_t parts = (token_tiles + tt - 1u) / tt;
+            if (5u * (parts * tt - token_tiles) > token_tiles) continue;
+            if (12u * quads * parts < enough[tt] * cus) continue;
+            if (tt == 4) return (int)launch_w4_matmul<4, 4>(a, vec, stream);
+            if (tt == 3) return (int)launch_w4_matmul<3, 4>(a, vec, stream);
+            if (tt == 2) return (int)launch_w4_matmul<2, 4>(a, vec, stream);
+            return (int)launch_w4_matmul<1, 4>(a, vec, stream);
         }
         // more than one a CU, or nearly one and few column tiles (their barriers)
         const uint64_t groups = pairs * token_tiles;
         if (groups > cus || (4u * groups >= 3u * cus && a.col_tiles <= 32u))
-            return (int)launch_w4_matmul<1, 1, 2>(a, vec, stream);
+            return (int)launch_w4_matmul<1, 2>(a, vec, stream);
     }
     if (a.row_tiles * token_tiles > cus) return (int)launch_w4<2>(a, vec, stream);
     return (int)launch_w4<1>(a, vec, stream);

@@ -138,6 +138,16 @@ def test_odd_columns(attn, gpu, T, N, K, group):
     product(attn, gpu, T, N, K, group, T, x_off=T % 3)
 
 
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("T,N,K", [
+    (16, 65600, 72), (7, 65540, 135), (60, 28700, 133), (64, 28720, 264), (33, 11008, 176),
+    (48, 10930, 171), (32, 12288, 168), (25, 12270, 143), (80, 11000, 104), (16, 12300, 392)])
+def test_workgroups_that_share_x(attn, gpu, T, N, K, group):
+    """Either side of the sizes from which workgroups take more rows or tokens."""
+    print(f"[case] T={T} N={N} K={K} group={group}", flush=True)
+    product(attn, gpu, T, N, K, group, T, residual="in place")
+
+
 def test_infinity_in_one_token_stays_there(attn, gpu):
     N, K = 40, 200
     codes, scales = weights(N, K, 32, 1)
