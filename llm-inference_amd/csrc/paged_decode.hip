@@ -268,8 +268,9 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_split(PagedSplitArgs
         len = clamp_len(a.lens[b], a.max_pages, a.page_size);
         u1 = (len + kUnit - 1u) / kUnit;
     } else {
-        uint32_t total = 0;
-        for (uint32_t b0 = 0; b0 < a.num_seqs; b0 += 64u)
+        const uint32_t len0 = len_of(a, lane), mine0 = line_units(len0), incl0 = wave_scan(mine0);
+        uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)incl0, 63);
+        for (uint32_t b0 = 64; b0 < a.num_seqs; b0 += 64u)
             total += (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(line_units(len_of(a, b0 + lane))), 63);
         // the line begins behind the first sequence's lead
         const uint32_t line = total > kLead ? total - kLead : 0u;
@@ -278,9 +279,13 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_split(PagedSplitArgs
         u = kLead + w * share;
         u1 = min(total, u + share);
         b = base = 0;
+        uint32_t mine_len = len0, mine = mine0, incl = incl0;
         for (uint32_t b0 = 0;; b0 += 64u) {
-            const uint32_t mine_len = len_of(a, b0 + lane), mine = line_units(mine_len);
-            const uint32_t incl = wave_scan(mine);
+            if (b0 > 0) {
+                mine_len = len_of(a, b0 + lane);
+                mine = line_units(mine_len);
+                incl = wave_scan(mine);
+            }
             const uint64_t past = __ballot(base + incl > u);
             if (past) {
                 const int at = (int)__builtin_ctzll(past);
