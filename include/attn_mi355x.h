@@ -286,10 +286,10 @@ int attn_qkv_gemm_rope_store_kv(const attn_f16_t* x, attn_f16_t* y, const attn_f
  * cache: a KVCache whose max_seq_len is num_pages * page_size is such a pool, layer
  * l's K and V its planes 2 l and 2 l + 1.  Row b of a page table, max_pages int32
  * entries, names the pages of sequence b in order: its cache row t is row t %
- * page_size of page table[b][t / page_size].  Entries past a sequence's length are
- * never read.  All of this is device memory, so lengths and tables may change
- * between replays of a captured call.  Sizes: num_pages * page_size and max_pages *
- * page_size at most 2^31 - 1; any page_size.  num_seqs, num_tokens or n == 0 is a
+ * page_size of page table[b][t / page_size].  Entries past a sequence's length
+ * name nothing, whatever they hold.  All of this is device memory, so lengths and
+ * tables may change between replays of a captured call.  Sizes: num_pages * page_size
+ * and max_pages * page_size at most 2^31 - 1; any page_size.  num_seqs, num_tokens or n == 0 is a
  * no-op.  Page numbers, sequence numbers, positions and lengths that are out of
  * range are caught on the device, as said at each call. */
 
@@ -319,7 +319,7 @@ int attn_paged_rope_store_kv(attn_f16_t* q, const attn_f16_t* k, const attn_f16_
  * page_size).  q rows are q_stride apart (0 = packed); out is packed
  * [num_seqs][num_heads][head_dim].  A sequence of length 0 or less keeps its
  * output row; one whose table names a page out of range gets NaN.  head_dim up to
- * 256; num_heads a multiple of num_kv_heads.  workspace:
+ * 256; num_heads a multiple of num_kv_heads; out must not overlap q.  workspace:
  * attn_paged_decode_workspace_bytes bytes, 16-byte aligned, any contents; calls
  * that share one must be ordered (one stream, or graphs replayed in order). */
 size_t attn_paged_decode_workspace_bytes(size_t num_seqs, size_t num_heads, size_t num_kv_heads,
@@ -402,8 +402,9 @@ int attn_w4_pack(const attn_f16_t* w, void* packed, attn_f16_t* scales, size_t o
 
 /* y[t] = W x[t] (+ residual[t]) for num_tokens tokens, fp16 in, fp32 accumulation, fp16
  * out: attn_qkv_decode and attn_out_proj_decode (beta 1) on 4-bit weights, for one token
- * or a batch.  x rows are x_stride apart, y and residual rows y_stride (0 = packed);
- * residual may be y, or NULL.  in_dim == 0: y = residual, or zeros. */
+ * or a batch.  x rows are x_stride apart, y and residual rows y_stride (0 = packed), y's
+ * without overlap.  residual may be y (the same address), or NULL; x must not overlap y.
+ * in_dim == 0: y = residual, or zeros. */
 int attn_w4_matvec(const attn_f16_t* x, attn_f16_t* y, const void* packed,
                    const attn_f16_t* scales, const attn_f16_t* residual, size_t num_tokens,
                    size_t in_dim, size_t out_dim, size_t group_size, size_t x_stride,

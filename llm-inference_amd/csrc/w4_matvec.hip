@@ -618,6 +618,7 @@ int attn_w4_matvec(const attn_f16_t* x, attn_f16_t* y, const void* packed,
                    size_t y_stride, hipStream_t stream) {
     if (num_tokens == 0 || out_dim == 0) return 0;
     if (!w4_sizes_ok(out_dim, in_dim, group_size) || num_tokens > 65535 || !y ||
+        (num_tokens > 1 && y_stride && y_stride < out_dim) ||
         (in_dim && (!x || !packed || !scales || ((uintptr_t)packed & 15u) ||
                     ((uintptr_t)scales & 7u))))
         return (int)hipErrorInvalidValue;

@@ -130,6 +130,12 @@ def test_w4_refusals(attn):
     assert lib.attn_w4_scale_count(17, 129, 0) == 0
 
 
+def test_w4_rows_of_y_that_overlap_are_refused(attn):
+    mv = lambda *a: attn.lib().attn_w4_matvec(*a, None)  # noqa: E731
+    assert mv(P, P, P, P, None, 2, 64, 64, 32, 0, 63) == INVALID
+    assert mv(P, P, P, P, P, 64, 0, 64, 32, 0, 8) == INVALID
+
+
 def test_wrappers_refuse_other_integers(attn):
     """Page numbers and lengths in 64 bits, or in another order, never reach the library."""
     import torch
