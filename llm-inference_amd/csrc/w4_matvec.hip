@@ -223,10 +223,11 @@ __device__ __forceinline__ f16x4 w4_lane_scale(u32x2 mine) {
 }
 
 // Few rows: R row tiles x 16 tokens a wave, the waves of a row tile split the columns, each
-// with its own x.  SPS: steps of 32 columns that share a scale at least (4: the group is a
-// multiple of 128; 2: of 64; 1).  The products of a scale's columns are summed by the MFMAs
+// with its own x, 4 X tokens of it (8 tokens, 2048 x 11008, groups of 128: 7.5 us with two
+// loads of x a tile, 8.7 with four).  SPS: steps of 32 columns that share a scale at least
+// (4: the group is a multiple of 128; 2: of 64; 1).  The products of a scale's columns are summed by the MFMAs
 // from zero, then scaled and added in fp32, so no product is rounded.
-template <int R, int SPS, bool VEC>
+template <int R, int SPS, int X, bool VEC>
 __global__ __launch_bounds__(64 * kW4Waves) void w4_matvec(W4Args a) {
     constexpr int kDepth = 2;  // column tiles in flight
     // a wave's x tile (16 tokens x 128 columns), then the waves' sums
@@ -263,13 +264,13 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matvec(W4Args a) {
         // bytes, as the MFMA operand wants it, took the load pipe twice as long), and turned
         // in LDS: row r's 16-byte chunk i lies at chunk i ^ r, so that the 16 rows of an
         // operand read cover all banks.
-        uint64_t x_at[4];  // elements; tokens past the last repeat it: nothing of theirs is stored
+        uint64_t x_at[X];  // elements; tokens past the last repeat it: nothing of theirs is stored
 #pragma unroll
-        for (uint32_t j = 0; j < 4; ++j)
+        for (uint32_t j = 0; j < X; ++j)
             x_at[j] = min(4u * j + gq, live - 1u) * a.x_stride + 8u * n;
         struct Stage {
             u32x4 w[R];
-            f16x8 x[4];
+            f16x8 x[X];
             u32x2 scale;  // rows 4 gq ..
         } st[kDepth];
         auto load = [&](uint32_t c, Stage& z) {
@@ -279,12 +280,12 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matvec(W4Args a) {
                 sc + w4_group(a, min(128u * c + 32u * (n >> 2), a.cols - 1u)) * sc_stride);
             const uint32_t k = 128u * c + 8u * n;
 #pragma unroll
-            for (uint32_t j = 0; j < 4; ++j)
+            for (uint32_t j = 0; j < X; ++j)
                 z.x[j] = w4_load_x<VEC>(rx, xb, x_at[j] + 128u * c, c, k, a.cols);
         };
         auto compute = [&](const Stage& z) {
 #pragma unroll
-            for (uint32_t j = 0; j < 4; ++j) {
+            for (uint32_t j = 0; j < X; ++j) {
                 const uint32_t r = 4u * j + gq;
                 s_mem.x[wave][16u * r + (n ^ r)] = z.x[j];
             }
@@ -320,22 +321,28 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matvec(W4Args a) {
     w4_store<16, R>(a, s_mem.part, t0, live);
 }
 
-template <int R, int SPS>
+template <int R, int SPS, int X>
 hipError_t launch_w4(const W4Args& a, bool vec, hipStream_t stream) {
     const uint32_t tiles = kW4Waves / a.split * R;
     const dim3 grid((a.row_tiles + tiles - 1u) / tiles, (a.tokens + 15u) / 16u);
+    const dim3 block(64 * kW4Waves);
     if (vec)
-        hipLaunchKernelGGL((w4_matvec<R, SPS, true>), grid, dim3(64 * kW4Waves), 0, stream, a);
+        hipLaunchKernelGGL((w4_matvec<R, SPS, X, true>), grid, block, 0, stream, a);
     else
-        hipLaunchKernelGGL((w4_matvec<R, SPS, false>), grid, dim3(64 * kW4Waves), 0, stream, a);
+        hipLaunchKernelGGL((w4_matvec<R, SPS, X, false>), grid, block, 0, stream, a);
     return hipGetLastError();
+}
+
+template <int R, int X>
+hipError_t launch_w4(const W4Args& a, bool vec, hipStream_t stream) {
+    if (a.group % 128 == 0) return launch_w4<R, 4, X>(a, vec, stream);
+    if (a.group % 64 == 0) return launch_w4<R, 2, X>(a, vec, stream);
+    return launch_w4<R, 1, X>(a, vec, stream);
 }
 
 template <int R>
 hipError_t launch_w4(const W4Args& a, bool vec, hipStream_t stream) {
-    if (a.group % 128 == 0) return launch_w4<R, 4>(a, vec, stream);
-    if (a.group % 64 == 0) return launch_w4<R, 2>(a, vec, stream);
-    return launch_w4<R, 1>(a, vec, stream);
+    return a.tokens <= 8 ? launch_w4<R, 2>(a, vec, stream) : launch_w4<R, 4>(a, vec, stream);
 }
 
 // Many rows and tokens: RW of the eight waves take row tiles of their own and share x, so
