@@ -6,9 +6,9 @@
 // page number out of range makes its sequence's output NaN: nothing is read for it.
 //
 // Bound by the K/V bytes, 4 * Hkv * D per key; by latency for short contexts.  Measured
-// (16/4 heads): 64 sequences of 100 to 16384 keys, heads of 128, 353 MB: split 65.1 us (5.4
-// TB/s) and join 4.2 traced, 70.8 a call; one of 32768: 12.1 and 3.9, 18.0; 32 of 20 to 4096
-// keys, heads of 64, 38 MB: 11.1 and 3.0, 14.2; one of 254: 5.0.
+// (16/4 heads): 64 sequences of 100 to 16384 keys, heads of 128, 353 MB: split 65.0 us (5.4
+// TB/s) and join 4.2 traced, 70.3 a call; one of 32768: 12.0 and 2.7, 16.9; 32 of 20 to 4096
+// keys, heads of 64, 38 MB: 10.9 and 3.0, 13.9; one of 254: 5.1.
 //
 // Split.  The lengths are known on the device only, and differ.  The keys of all
 // sequences, in units of 32 keys and one after the other, make one line of units; each

@@ -14,7 +14,7 @@
 // zero in rows past the matrix.
 //
 // Bound by the weights' bytes for a few tokens and many rows (one token, 128256 x 2048: 135.7
-// MB in 26.7 us, 5.1 TB/s), by latency for few rows (2048 x 2048: 3.2 us).  For a batch
+// MB in 25.8 us, 5.3 TB/s), by latency for few rows (2048 x 2048: 3.2 us).  For a batch
 // the load pipe and the unpacking bound it (33 tokens, 2048 x 11008, groups of 32: 12.6 us,
 // of which the weights' 11.3 MB would take 2.7): each workgroup reads its tokens' whole rows
 // of x, about 9 ns a KiB and CU wherever they lie, and the vector instructions take half
@@ -52,7 +52,7 @@ struct W4Args {
 // less 1032, or over 16 and less 72, both exact in fp16.  The constants live in registers
 // (hidden from the compiler), so that mask and or are one v_and_or_b32, which takes no
 // literals: 9 instructions a word, 13 otherwise (33 tokens, 2048 x 11008,
-// groups of 32: 14.4 us against 15.1).
+// groups of 32: 13.0 us against 13.9).
 struct W4Consts {
     uint32_t low, high, one;
     __device__ W4Consts() : low(0x000f000fu), high(0x00f000f0u), one(0x64006400u) {
@@ -73,8 +73,8 @@ __device__ __forceinline__ f16x8 w4_values(uint32_t word, const W4Consts& k) {
     return f16x8{v0[0], v0[1], v1[0], v1[1], v2[0], v2[1], v3[0], v3[1]};
 }
 
-// 16 bytes of codes per lane.  Without the non-temporal hint: 16 tokens, 12000 x 12000 22.8
-// us against 28.1 with it, one token, 128256 x 2048 (HBM-cold) level.
+// 16 bytes of codes per lane.  Without the non-temporal hint: 16 tokens, 12000 x 12000 23.4
+// us against 28.0 with it, one token, 128256 x 2048 (HBM-cold) level.
 __device__ __forceinline__ u32x4 w4_load(BufRsrc rows, uint32_t byte_off) {
     return __builtin_bit_cast(u32x4,
                               __builtin_amdgcn_raw_buffer_load_b128(rows, (int)byte_off, 0, 0));
@@ -508,7 +508,7 @@ hipError_t launch_w4_narrow(const W4Args& a, bool vec, hipStream_t stream) {
 }
 
 // Waves per row tile, no more than there are column tiles.  Narrow: enough for eight waves
-// a CU.  Otherwise as many as there are (33 tokens, 2048 x 11008: 14 us with eight, 23 with
+// a CU.  Otherwise as many as there are (33 tokens, 2048 x 11008: 13 us with eight, 22 with
 // four).
 uint32_t w4_split(uint32_t row_tiles, uint32_t col_tiles, bool narrow, int cus) {
     uint32_t split = 1;
