@@ -43,6 +43,7 @@ class PagedKVCache {
                             attn_paged_decode_workspace_bytes(max_seqs_, decode_heads_,
                                                               num_kv_heads_, head_dim_)));
         HIP_CHECK(hipMemset(state_, 0, words * sizeof(int32_t)));
+        HIP_CHECK(hipStreamSynchronize(nullptr));  // zero for calls on any stream
     }
     ~PagedKVCache() {
         (void)hipFree(pool_);

@@ -334,6 +334,12 @@ def _ints(x, what) -> Optional[int]:
     raise AttnError(f"{what} must be a contiguous int32 tensor, got {x.dtype}")
 
 
+def _entries(x, what, n):
+    if x is not None and not isinstance(x, int) and x.numel() < n:
+        raise AttnError(f"{what} has {x.numel()} entries, needs {n}")
+    return x
+
+
 # the current device's index, for callers that know CUDA to be initialised
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
@@ -545,6 +551,9 @@ class PagedKVCache:
         self._pages_ws = pages_workspace(max_seqs, num_pages, device)
         self._decode_ws = {}
 
+    def _per_seq(self, x, what):
+        return _entries(x, what, self.max_seqs)
+
     def k(self, layer):
         return self.pool[2 * layer]
 
@@ -554,19 +563,21 @@ class PagedKVCache:
     def grow(self, tokens, stream=None):
         """Each sequence by tokens[b] (int32 [max_seqs])."""
         pages_grow(self.pool, 2 * self.num_layers, self.page_elems, self.page_table,
-                   self.seq_lens, tokens, self.ref_counts, self.status, self.max_seqs,
-                   self.max_pages, self.num_pages, self.page_size, self._pages_ws, stream=stream)
+                   self.seq_lens, self._per_seq(tokens, "grow"), self.ref_counts, self.status,
+                   self.max_seqs, self.max_pages, self.num_pages, self.page_size,
+                   self._pages_ws, stream=stream)
 
     def free(self, keep_lens=None, stream=None):
         """Each sequence cut to keep_lens[b] tokens (None: all to 0; -1: left alone)."""
         pages_free(self.page_table, self.seq_lens, self.ref_counts, self.max_seqs,
-                   self.max_pages, self.num_pages, self.page_size, keep_lens, stream)
+                   self.max_pages, self.num_pages, self.page_size,
+                   self._per_seq(keep_lens, "keep_lens"), stream)
 
     def fork(self, parents, stream=None):
         """The empty sequence i becomes a fork of sequence parents[i] (-1: left alone)."""
-        pages_fork(self.page_table, self.seq_lens, self.page_table, self.seq_lens, parents,
-                   self.ref_counts, self.max_seqs, self.max_seqs, self.max_pages,
-                   self.num_pages, self.page_size, stream)
+        pages_fork(self.page_table, self.seq_lens, self.page_table, self.seq_lens,
+                   self._per_seq(parents, "parents"), self.ref_counts, self.max_seqs,
+                   self.max_seqs, self.max_pages, self.num_pages, self.page_size, stream)
 
     def compact(self, stream=None):
         pages_compact(self.pool, 2 * self.num_layers, self.page_elems, self.page_table,
@@ -578,6 +589,8 @@ class PagedKVCache:
                q_stride=0, k_stride=0, apply_rotation=True, q_out=None, seq_ids=None,
                stream=None):
         """paged_rope_store_kv into a layer's pages."""
+        _entries(positions, "positions", num_tokens)
+        _entries(seq_ids, "seq_ids", num_tokens)
         paged_rope_store_kv(q, k, v, self.k(layer), self.v(layer), cos, sin, self.page_table,
                             positions, num_tokens, self.max_seqs, self.max_pages,
                             self.num_pages, self.page_size, max_seq_len, num_heads,
@@ -586,7 +599,8 @@ class PagedKVCache:
 
     def decode(self, layer, q, out, num_heads, q_stride=0, stream=None):
         """paged_decode of one token per sequence over a layer's pages.  Calls on one
-        cache share a workspace and must be ordered."""
+        cache share a workspace and must be ordered; the first with a number of heads
+        allocates it, so not inside a capture."""
         if num_heads not in self._decode_ws:
             self._decode_ws[num_heads] = paged_decode_workspace(
                 self.max_seqs, num_heads, self.num_kv_heads, self.head_dim, self.pool.device)

@@ -136,6 +136,18 @@ def test_w4_rows_of_y_that_overlap_are_refused(attn):
     assert mv(P, P, P, P, P, 64, 0, 64, 32, 0, 8) == INVALID
 
 
+def test_cache_refuses_lists_that_are_too_short(attn):
+    import torch
+    cache = attn.PagedKVCache(1, 8, 4, 1, 8, 3, 2, device="cpu")
+    short = torch.zeros(2, dtype=torch.int32)
+    for call in (cache.grow, cache.free, cache.fork):
+        with pytest.raises(attn.AttnError, match="2 entries, needs 3"):
+            call(short)
+    for lists in ((short, None), (torch.zeros(3, dtype=torch.int32), short)):
+        with pytest.raises(attn.AttnError, match="2 entries, needs 3"):
+            cache.append(0, P, P, P, P, P, lists[0], 3, 1, 8, seq_ids=lists[1])
+
+
 def test_wrappers_refuse_other_integers(attn):
     """Page numbers and lengths in 64 bits, or in another order, never reach the library."""
     import torch
