@@ -110,7 +110,7 @@ __device__ __forceinline__ uint32_t w4_group(const W4Args& a, uint32_t k) {
 }
 
 // Sums of the waves that share a row tile: `part` waves (a power of two) of the workgroup's
-// eight, wave-contiguous.  s_part is [wave][tokens][17].
+// eight, wave-contiguous.  s_part is [wave][tokens][rows + 1].
 template <int TOKENS, int R>
 __device__ __forceinline__ void w4_store(const W4Args& a, const float (*s_part)[TOKENS][16 * R + 1],
                                          uint32_t t0, uint32_t live) {
