@@ -345,15 +345,17 @@ hipError_t launch_w4(const W4Args& a, bool vec, hipStream_t stream) {
     return a.tokens <= 8 ? launch_w4<R, 2>(a, vec, stream) : launch_w4<R, 4>(a, vec, stream);
 }
 
-// Many rows and tokens: RW of the eight waves take row tiles of their own and share x, so
-// that a workgroup reads x once for 16 RW rows and unpacks codes once for 16 TT tokens; the
-// 8 / RW groups of waves split the columns.  x goes through two LDS tiles in turn: each wave of a group loads its part of the
-// next tile into registers, and one barrier a column tile parts the writes from the reads.
-// Tiles past the last column are zeros through the range checks, so every wave runs the same
-// number of rounds.
-template <int TT, int RW, int SPS, bool VEC>
-__global__ __launch_bounds__(64 * kW4Waves) void w4_matmul(W4Args a) {
-    constexpr uint32_t kGroups = kW4Waves / RW;
+// Many rows and tokens: RW of the W waves take row tiles of their own and share x, so that a
+// workgroup reads x once for 16 RW rows and unpacks codes once for 16 TT tokens; the W / RW
+// groups of waves split the columns.  x goes through two LDS tiles in turn: each wave of a
+// group loads its part of the next tile into registers, and one barrier a column tile parts
+// the writes from the reads.  Tiles past the last column are zeros through the range checks,
+// so every wave runs the same number of rounds.  Sixteen waves where a workgroup has its CU
+// to itself: eight leave it waiting for the barrier (64 tokens, 12000 x 12000: 40.6 us against
+// 51.2; but two workgroups of sixteen do not fit a CU's registers).
+template <int TT, int RW, int W, int SPS, bool VEC>
+__global__ __launch_bounds__(64 * W) void w4_matmul(W4Args a) {
+    constexpr uint32_t kGroups = W / RW;
     constexpr int kLoads = 4 * TT / RW;  // of a wave for a tile of x
     static_assert(kLoads * RW == 4 * TT);
     constexpr uint32_t kRows = 16 * RW;
@@ -404,11 +406,11 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matmul(W4Args a) {
     f32x4 acc[TT];
 #pragma unroll
     for (int tt = 0; tt < TT; ++tt) acc[tt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    // Groups of 32, three token tiles and more: a step's sums are scaled after the next
-    // step's products, which hide the MFMAs' latency (48 tokens, 16384 x 4096: 18.3 us
-    // against 22.9; with wider groups the compiler's order is the better one, 15.4 against
-    // 17.2 with groups of 64).
-    constexpr bool kLate = SPS == 1 && TT > 2;
+    // Groups of 32, three token tiles and more or sixteen waves: a step's sums are scaled
+    // after the next step's products, which hide the MFMAs' latency (48 tokens, 16384 x 4096,
+    // eight waves 18.3 us against 22.9; 32 tokens, 12000 x 12000, sixteen 31.8 against 38.3; with
+    // wider groups the compiler's order is the better one, 15.4 against 17.2 with groups of 64).
+    constexpr bool kLate = SPS == 1 && (TT > 2 || W == 16);
     auto compute = [&](const f16x8 (*x)[256], const Weights& z) {
         f32x4 part[kLate ? 2 : 1][TT];
         auto add = [&]<int g>() {
@@ -437,6 +439,8 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matmul(W4Args a) {
                 __builtin_amdgcn_sched_barrier(0);
             }
             if constexpr (!kLate && s % SPS == SPS - 1) add.template operator()<g>();
+            if constexpr (W == 16 && TT == 3 && SPS == 4)
+                __builtin_amdgcn_sched_barrier(0);  // else 129 registers
         };
         step.template operator()<0>();
         step.template operator()<1>();
@@ -466,7 +470,7 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matmul(W4Args a) {
         for (int r = 0; r < 4; ++r)
             s_mem.part[kg][16 * tt + n][16u * rg + 4u * gq + r] = acc[tt][r];
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < live * kRows; i += 64u * kW4Waves) {
+    for (uint32_t i = threadIdx.x; i < live * kRows; i += 64u * W) {
         const uint32_t t = i / kRows, r = i % kRows, row = blockIdx.x * kRows + r;
         if (row >= a.rows) continue;
         float sum = 0.f;
@@ -478,23 +482,25 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matmul(W4Args a) {
     }
 }
 
-template <int TT, int RW, bool VEC>
+template <int TT, int RW, int W, bool VEC>
 hipError_t launch_w4_matmul(const W4Args& a, hipStream_t stream) {
     const dim3 grid((a.row_tiles + RW - 1u) / RW, (a.tokens + 16u * TT - 1u) / (16u * TT));
-    const dim3 block(64 * kW4Waves);
+    const dim3 block(64 * W);
     if (a.group % 128 == 0)
-        hipLaunchKernelGGL((w4_matmul<TT, RW, 4, VEC>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((w4_matmul<TT, RW, W, 4, VEC>), grid, block, 0, stream, a);
     else if (a.group % 64 == 0)
-        hipLaunchKernelGGL((w4_matmul<TT, RW, 2, VEC>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((w4_matmul<TT, RW, W, 2, VEC>), grid, block, 0, stream, a);
+    else if constexpr (W == 8 || TT < 4 || VEC)
+        hipLaunchKernelGGL((w4_matmul<TT, RW, W, 1, VEC>), grid, block, 0, stream, a);
     else
-        hipLaunchKernelGGL((w4_matmul<TT, RW, 1, VEC>), grid, block, 0, stream, a);
+        return hipErrorInvalidValue;  // not asked for
     return hipGetLastError();
 }
 
-template <int TT, int RW>
+template <int TT, int RW, int W>
 hipError_t launch_w4_matmul(const W4Args& a, bool vec, hipStream_t stream) {
-    return vec ? launch_w4_matmul<TT, RW, true>(a, stream)
-               : launch_w4_matmul<TT, RW, false>(a, stream);
+    return vec ? launch_w4_matmul<TT, RW, W, true>(a, stream)
+               : launch_w4_matmul<TT, RW, W, false>(a, stream);
 }
 
 hipError_t launch_w4_narrow(const W4Args& a, bool vec, hipStream_t stream) {
@@ -656,46 +662,59 @@ int attn_w4_matvec(const attn_f16_t* x, attn_f16_t* y, const void* packed,
                      a.x_stride < (1ull << 31) && x_range * 2 < kDead;
     if (a.tokens <= 4) return (int)launch_w4_narrow(a, vec, stream);
     // Which kernel, by the workgroups it makes.  P r: own x for every wave, r row tiles; S t w:
-    // x shared by w waves of a row tile each, t token tiles (us in a graph, groups of 64;
-    // tokens x rows x columns, CUs 256):
-    //                       P 1    P 2   S 1 2   S 1 4   S 2 4   S 3 4   S 4 4
-    //  16 x 4096 x 4096     5.4    6.1    6.6     9.8    10.9    13.6    16.6
-    //  16 x 8192 x 8192    12.4   10.7   12.3    18.3    20.2    24.7    30.4
-    //  16 x 11008 x 2048    7.0    6.3    5.7     6.7     7.3     8.6    10.0
-    //  16 x 128256 x 2048  49.8   38.0   33.6    29.4    37.3    46.7    55.5
-    //  33 x 2048 x 2048     4.7    4.3    4.1     5.2     6.5     8.2     9.6
-    //  64 x 2048 x 11008   14.8   12.0   15.0    23.4    26.3    33.6    40.6
-    //  32 x 8192 x 8192    20.8   15.5   14.4    18.3    20.1    24.8    30.7
-    //  32 x 11008 x 2048           8.1    7.2     8.4     7.4     8.7    10.1
-    //  32 x 24000 x 2048   18.1   14.8   12.4    11.7    10.2    12.5    14.8
-    //  48 x 8192 x 4096    16.3   13.2   11.5    12.7    11.9    14.4    16.8
-    //  48 x 11008 x 2048          11.3    9.9    10.2     9.8     8.9    10.1
-    //  48 x 16384 x 4096          23.4   20.2    18.4    17.2    15.3    18.1
-    //  64 x 8192 x 8192    36.4   26.5   24.8    22.6    20.5    26.3    30.2
-    //  64 x 12000 x 12000  82.9   57.6   56.0    50.0    43.8    56.1    47.6
-    //  64 x 30000 x 2048          32.2   26.3    26.0    19.4    24.2    16.9
-    //  64 x 128256 x 2048   160    122    106    91.9    66.1    90.5    63.2
-    //  96 x 6000 x 4096    22.8   18.9   16.9    17.6    16.6    14.7    17.4
+    // x shared by w waves of a row tile each, t token tiles, eight waves in all; L t: S t 4 with
+    // sixteen (us in a graph, groups of 64; tokens x rows x columns, CUs 256):
+    //                       P 1   P 2  S 1 2  S 1 4  S 2 4  S 3 4  S 4 4   L 2   L 3   L 4
+    //  16 x 4096 x 4096     5.4   6.1   6.6    9.8   10.9   13.6   16.6
+    //  16 x 8192 x 8192    12.4  10.7  12.3   18.3   20.2   24.7   30.4
+    //  16 x 11008 x 2048    7.0   6.3   5.7    6.7    7.3    8.6   10.0   6.6   7.7   8.8
+    //  16 x 128256 x 2048  49.8  38.0  33.6   29.4   37.3   46.7   55.5
+    //  33 x 2048 x 2048     4.7   4.3   4.1    5.2    6.5    8.2    9.6
+    //  64 x 2048 x 11008   14.8  12.0  15.0   23.4   26.3   33.6   40.6
+    //  32 x 8192 x 8192    20.9  15.5  14.7   18.5   20.3   24.8   30.7  17.6  20.6  24.4
+    //  64 x 4096 x 4096    11.8   9.3   8.7   10.0   11.1   14.2   16.7   9.8  12.0  14.2
+    //  32 x 11008 x 2048          8.1   7.1    8.4    7.3    8.3    9.9   6.7   7.7   9.0
+    //  32 x 24000 x 2048   18.1  14.8  12.4   11.7   10.2   12.5   14.8
+    //  48 x 8192 x 4096    16.3  13.2  12.5   12.7   13.0   14.5   17.0  11.4  12.7  14.7
+    //  33 x 16384 x 2048         13.4  11.4   10.2    9.9    8.9   10.2  11.9   8.3   9.2
+    //  64 x 6000 x 4096    17.8  14.4  11.8   14.1   12.2   14.0   16.6  10.7  12.6  14.5
+    //  64 x 8192 x 8192    36.4  26.5  25.4   22.6   21.3   25.2   29.4  18.6  21.7  25.2
+    //  64 x 9000 x 4096                19.2   18.1   16.6   20.0   16.6  19.2  22.0  14.5
+    //  64 x 20000 x 2048   27.8  22.4  18.2   19.9   13.6   19.3   15.8  18.2  20.6  17.2
+    //  64 x 30000 x 2048         32.2  26.3   26.0   19.4   24.2   16.9
+    //  64 x 128256 x 2048   160   122   106   91.9   66.1   90.5   63.2
+    //  96 x 6000 x 4096    22.8  18.9  17.4   17.6   16.9   14.1   17.0  19.5  12.6  14.9
     const uint64_t cus = (uint32_t)device_cu_count(device);
     const uint64_t token_tiles = (a.tokens + 15u) / 16u;
     if (in_dim > 0) {
         const uint64_t quads = (a.row_tiles + 3u) / 4u, pairs = (a.row_tiles + 1u) / 2u;
-        // the most token tiles that fit the tokens (a fifth more at most) and leave enough
-        // workgroups, in twelfths of the CUs
-        const uint64_t enough[5] = {0, 48, 9, 8, 21};
+        // Sixteen waves, a workgroup a CU at most: the fewest token tiles that make no more of
+        // them (S 1 2 has more, but two a CU are as fast).
+        if (pairs * token_tiles > 2u * cus && token_tiles > 1) {
+            if (quads * ((token_tiles + 1u) / 2u) <= cus)
+                return (int)launch_w4_matmul<2, 4, 16>(a, vec, stream);
+            if (quads * ((token_tiles + 2u) / 3u) <= cus)
+                return (int)launch_w4_matmul<3, 4, 16>(a, vec, stream);
+            // (groups of 32 with rows of x at any element would spill 22 registers)
+            if (quads * ((token_tiles + 3u) / 4u) <= cus && (vec || group_size % 64 == 0))
+                return (int)launch_w4_matmul<4, 4, 16>(a, vec, stream);
+        }
+        // Eight: the most token tiles that fit the tokens (a fifth more at most) and leave
+        // enough workgroups, in quarters of the CUs.
+        const uint64_t enough[5] = {0, 16, 4, 4, 7};
         for (uint64_t tt = std::min<uint64_t>(4, token_tiles); tt > 0; --tt) {
             const uint64_t parts = (token_tiles + tt - 1u) / tt;
             if (5u * (parts * tt - token_tiles) > token_tiles) continue;
-            if (12u * quads * parts < enough[tt] * cus) continue;
-            if (tt == 4) return (int)launch_w4_matmul<4, 4>(a, vec, stream);
-            if (tt == 3) return (int)launch_w4_matmul<3, 4>(a, vec, stream);
-            if (tt == 2) return (int)launch_w4_matmul<2, 4>(a, vec, stream);
-            return (int)launch_w4_matmul<1, 4>(a, vec, stream);
+            if (4u * quads * parts < enough[tt] * cus) continue;
+            if (tt == 4) return (int)launch_w4_matmul<4, 4, 8>(a, vec, stream);
+            if (tt == 3) return (int)launch_w4_matmul<3, 4, 8>(a, vec, stream);
+            if (tt == 2) return (int)launch_w4_matmul<2, 4, 8>(a, vec, stream);
+            return (int)launch_w4_matmul<1, 4, 8>(a, vec, stream);
         }
         // more than one a CU, or nearly one and few column tiles (their barriers)
         const uint64_t groups = pairs * token_tiles;
         if (groups > cus || (4u * groups >= 3u * cus && a.col_tiles <= 32u))
-            return (int)launch_w4_matmul<1, 2>(a, vec, stream);
+            return (int)launch_w4_matmul<1, 2, 8>(a, vec, stream);
     }
     if (a.row_tiles * token_tiles > cus) return (int)launch_w4<2>(a, vec, stream);
     return (int)launch_w4<1>(a, vec, stream);
