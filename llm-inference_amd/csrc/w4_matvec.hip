@@ -109,14 +109,14 @@ __device__ __forceinline__ uint32_t w4_group(const W4Args& a, uint32_t k) {
     return __umulhi(k >> 5 << 1, a.group_mul);
 }
 
-// Sums of the waves that share a row tile: `part` waves (a power of two) of the workgroup's
-// eight, wave-contiguous.  s_part is [wave][tokens][rows + 1].
-template <int TOKENS, int R>
+// Sums of the waves that share a row tile: a.split (a power of two) of the workgroup's W,
+// neighbours.  s_part is [wave][tokens][rows + 1].
+template <int TOKENS, int R, int W>
 __device__ __forceinline__ void w4_store(const W4Args& a, const float (*s_part)[TOKENS][16 * R + 1],
                                          uint32_t t0, uint32_t live) {
-    const uint32_t tiles = kW4Waves / a.split, first = blockIdx.x * tiles;
+    const uint32_t tiles = W / a.split, first = blockIdx.x * tiles;
     const uint32_t per_tile = live * 16u * R;
-    for (uint32_t i = threadIdx.x; i < tiles * per_tile; i += 64u * kW4Waves) {
+    for (uint32_t i = threadIdx.x; i < tiles * per_tile; i += 64u * W) {
         const uint32_t tile = i / per_tile, j = i - tile * per_tile;
         const uint32_t t = j / (16u * R), r = j % (16u * R), row = (first + tile) * 16u * R + r;
         if (row >= a.rows) continue;
@@ -209,7 +209,7 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matvec_narrow(W4Args a) {
         if (step == 0) s_part[wave][n][4u * gq + r] = v;
     }
     __syncthreads();
-    w4_store<4, 1>(a, s_part, 0, a.tokens);
+    w4_store<4, 1, kW4Waves>(a, s_part, 0, a.tokens);
 }
 
 // the scales that lane L of a row of 16 lanes loaded, in all of them
@@ -227,19 +227,19 @@ __device__ __forceinline__ f16x4 w4_lane_scale(u32x2 mine) {
 // loads of x a tile, 8.7 with four).  SPS: steps of 32 columns that share a scale at least
 // (4: the group is a multiple of 128; 2: of 64; 1).  The products of a scale's columns are summed by the MFMAs
 // from zero, then scaled and added in fp32, so no product is rounded.
-template <int R, int SPS, int X, bool VEC>
-__global__ __launch_bounds__(64 * kW4Waves) void w4_matvec(W4Args a) {
+template <int R, int SPS, int X, int W, bool VEC>
+__global__ __launch_bounds__(64 * W) void w4_matvec(W4Args a) {
     constexpr int kDepth = 2;  // column tiles in flight
     // a wave's x tile (16 tokens x 128 columns), then the waves' sums
     union Shared {
-        f16x8 x[kW4Waves][256];
-        float part[kW4Waves][16][16 * R + 1];
+        f16x8 x[W][256];
+        float part[W][16][16 * R + 1];
     };
     __shared__ __attribute__((aligned(16))) Shared s_mem;
     const uint32_t lane = threadIdx.x & 63u;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t n = lane & 15u, gq = lane >> 4;
-    const uint32_t rt = (blockIdx.x * kW4Waves + wave) / a.split * R;
+    const uint32_t rt = (blockIdx.x * W + wave) / a.split * R;
     const uint32_t first = wave & (a.split - 1u);
     const uint32_t t0 = blockIdx.y * 16u;
     const uint32_t live = min(a.tokens - t0, 16u);
@@ -318,31 +318,41 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_matvec(W4Args a) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) s_mem.part[wave][n][16 * q + 4u * gq + r] = acc[q][r];
     __syncthreads();
-    w4_store<16, R>(a, s_mem.part, t0, live);
+    w4_store<16, R, W>(a, s_mem.part, t0, live);
 }
 
 template <int R, int SPS, int X>
-hipError_t launch_w4(const W4Args& a, bool vec, hipStream_t stream) {
+hipError_t launch_w4(W4Args a, bool vec, uint64_t cus, hipStream_t stream) {
     const uint32_t tiles = kW4Waves / a.split * R;
     const dim3 grid((a.row_tiles + tiles - 1u) / tiles, (a.tokens + 15u) / 16u);
-    const dim3 block(64 * kW4Waves);
-    if (vec)
-        hipLaunchKernelGGL((w4_matvec<R, SPS, X, true>), grid, block, 0, stream, a);
-    else
-        hipLaunchKernelGGL((w4_matvec<R, SPS, X, false>), grid, block, 0, stream, a);
+    // Sixteen waves where a workgroup has its CU to itself and each wave four column tiles (33
+    // tokens, 2048 x 11008, groups of 32: 12.1 us against 13.2; level at 4096 columns).  Rows of
+    // x at any element would spill.
+    if (vec && a.col_tiles >= 64 && (uint64_t)grid.x * grid.y <= cus) {
+        a.split = 16;
+        hipLaunchKernelGGL((w4_matvec<R, SPS, X, 16, true>),
+                           dim3((a.row_tiles + R - 1u) / R, grid.y), dim3(64 * 16), 0, stream, a);
+    } else if (vec) {
+        hipLaunchKernelGGL((w4_matvec<R, SPS, X, kW4Waves, true>), grid, dim3(64 * kW4Waves), 0,
+                           stream, a);
+    } else {
+        hipLaunchKernelGGL((w4_matvec<R, SPS, X, kW4Waves, false>), grid, dim3(64 * kW4Waves), 0,
+                           stream, a);
+    }
     return hipGetLastError();
 }
 
 template <int R, int X>
-hipError_t launch_w4(const W4Args& a, bool vec, hipStream_t stream) {
-    if (a.group % 128 == 0) return launch_w4<R, 4, X>(a, vec, stream);
-    if (a.group % 64 == 0) return launch_w4<R, 2, X>(a, vec, stream);
-    return launch_w4<R, 1, X>(a, vec, stream);
+hipError_t launch_w4(const W4Args& a, bool vec, uint64_t cus, hipStream_t stream) {
+    if (a.group % 128 == 0) return launch_w4<R, 4, X>(a, vec, cus, stream);
+    if (a.group % 64 == 0) return launch_w4<R, 2, X>(a, vec, cus, stream);
+    return launch_w4<R, 1, X>(a, vec, cus, stream);
 }
 
 template <int R>
-hipError_t launch_w4(const W4Args& a, bool vec, hipStream_t stream) {
-    return a.tokens <= 8 ? launch_w4<R, 2>(a, vec, stream) : launch_w4<R, 4>(a, vec, stream);
+hipError_t launch_w4(const W4Args& a, bool vec, uint64_t cus, hipStream_t stream) {
+    return a.tokens <= 8 ? launch_w4<R, 2>(a, vec, cus, stream)
+                         : launch_w4<R, 4>(a, vec, cus, stream);
 }
 
 // Many rows and tokens: RW of the W waves take row tiles of their own and share x, so that a
@@ -716,8 +726,8 @@ int attn_w4_matvec(const attn_f16_t* x, attn_f16_t* y, const void* packed,
         if (groups > cus || (4u * groups >= 3u * cus && a.col_tiles <= 32u))
             return (int)launch_w4_matmul<1, 2, 8>(a, vec, stream);
     }
-    if (a.row_tiles * token_tiles > cus) return (int)launch_w4<2>(a, vec, stream);
-    return (int)launch_w4<1>(a, vec, stream);
+    if (a.row_tiles * token_tiles > cus) return (int)launch_w4<2>(a, vec, cus, stream);
+    return (int)launch_w4<1>(a, vec, cus, stream);
 }
 
 }  // extern "C"

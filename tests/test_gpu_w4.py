@@ -148,6 +148,15 @@ def test_workgroups_that_share_x(attn, gpu, T, N, K, group):
     product(attn, gpu, T, N, K, group, T, residual="in place")
 
 
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("T,N,K", [(16, 40, 8200), (7, 33, 8192), (8, 300, 8064), (5, 17, 8072),
+                                   (33, 2050, 8328), (64, 2040, 8208), (64, 2050, 8208)])
+def test_many_columns(attn, gpu, T, N, K, group):
+    """Few rows of many columns, split between more waves."""
+    print(f"[case] T={T} N={N} K={K} group={group}", flush=True)
+    product(attn, gpu, T, N, K, group, T, x_pad=8, residual="apart")
+
+
 def test_infinity_in_one_token_stays_there(attn, gpu):
     N, K = 40, 200
     codes, scales = weights(N, K, 32, 1)
