@@ -15,7 +15,7 @@
 //
 // Bound by the weights' bytes for a few tokens and many rows (one token, 128256 x 2048: 135.7
 // MB in 25.8 us, 5.3 TB/s), by latency for few rows (2048 x 2048: 3.2 us).  For a batch
-// the load pipe and the unpacking bound it (33 tokens, 2048 x 11008, groups of 32: 12.6 us,
+// the load pipe and the unpacking bound it (33 tokens, 2048 x 11008, groups of 32: 12.0 us,
 // of which the weights' 11.3 MB would take 2.7): each workgroup reads its tokens' whole rows
 // of x, about 9 ns a KiB and CU wherever they lie, and the vector instructions take half
 // the time.  Many rows share those reads between the waves of a workgroup; for few rows,
@@ -52,7 +52,7 @@ struct W4Args {
 // less 1032, or over 16 and less 72, both exact in fp16.  The constants live in registers
 // (hidden from the compiler), so that mask and or are one v_and_or_b32, which takes no
 // literals: 9 instructions a word, 13 otherwise (33 tokens, 2048 x 11008,
-// groups of 32: 13.0 us against 13.9).
+// groups of 32: 13.0 us against 13.9 with eight waves).
 struct W4Consts {
     uint32_t low, high, one;
     __device__ W4Consts() : low(0x000f000fu), high(0x00f000f0u), one(0x64006400u) {
